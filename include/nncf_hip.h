@@ -569,6 +569,63 @@ int nncf_eval_whole(nncf_model* m, const int32_t* d_uid, int64_t n_users, const 
                     const int32_t* d_truth_ptr, const int32_t* d_truth_idx, int32_t topk, float* d_metrics,
                     int32_t* d_valid, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * The catalogue head (no reference counterpart: its losses sample their negatives, objectives.py:35-220, and its scores are
+ * fp32, objectives.py:310): the softmax cross entropy over the WHOLE item table, and scores from rows held in 8 bits.
+ * ---------------------------------------------------------------------------------- */
+typedef enum { NNCF_F32 = 0, NNCF_F16 = 1, NNCF_BF16 = 2 } nncf_dtype;
+typedef enum { NNCF_NONE = 0, NNCF_MEAN = 1, NNCF_SUM = 2 } nncf_reduction;
+
+/* Softmax cross entropy of n rows over c items, with its gradients:
+ *   z_ij = scale * <rows_i, table_j> + bias_j,   lse_i = log sum_j exp z_ij,   loss_i = weight_i * (lse_i - z_i,target_i)
+ *   reduction NNCF_SUM: loss[0] = sum of loss_i; NNCF_MEAN: that over the number of rows with a target (0 rows: loss 0);
+ *   NNCF_NONE: loss[n].  d_rows[n][dim], d_table[c][dim], d_bias[c]: the gradients of loss[0] (NNCF_NONE: of the sum of loss_i,
+ *   so that weight carries an upstream gradient).  The n x c values are never stored; sums are kept in 32 bits, nothing is added
+ *   in a varying order.
+ * - rows, table, d_rows, d_table hold elements of `dtype`; strides in elements, any alignment of their own type (16-byte aligned
+ *   rows of a multiple of 4 elements are read fastest); the gradients are contiguous.  dim <= 128 (any), as every row of this library.
+ * - target_i < 0: the row takes no part (loss 0, lse 0, gradient 0, its values are not used).  target_i >= c: NaN loss and gradients.
+ * - bias_j = -inf: item j is left out (its row is not used, its gradient is 0).  A row whose target is left out, or that has no item
+ *   left, has loss +inf and no gradient.
+ * - weight (NULL = 1): any finite value, 0 and negative ones too.  bias NULL = 0.
+ * - d_rows and d_table: both or neither (loss only); d_bias NULL or with a bias.  1 <= n, c <= 128 * 65535.
+ * The workspace (256-byte aligned, nncf_softmax_xent_ws_bytes; -1 for a shape that is refused) holds nothing between calls; calls
+ * that may run at the same time need one each. */
+typedef struct nncf_xent {
+  const void* rows;       /* [n] rows of dim elements */
+  const void* table;      /* [c] */
+  const int32_t* target;  /* [n] */
+  const float* bias;      /* [c] or NULL */
+  const float* weight;    /* [n] or NULL */
+  float* loss;            /* [1], or [n] with NNCF_NONE */
+  float* lse;             /* [n] */
+  void* d_rows;           /* [n][dim] or NULL */
+  void* d_table;          /* [c][dim] or NULL */
+  float* d_bias;          /* [c] or NULL */
+  int64_t n, c;
+  int64_t rows_stride, table_stride;
+  int32_t dim;
+  int32_t dtype;          /* nncf_dtype */
+  int32_t reduction;      /* nncf_reduction */
+  float scale;
+} nncf_xent;
+int64_t nncf_softmax_xent_ws_bytes(int64_t n, int64_t c, int32_t dim, int32_t dtype, int32_t with_grad);
+int nncf_softmax_xent(const nncf_xent* x, void* d_ws, int64_t ws_bytes, void* stream);
+
+/* Rows in 8 bits: code = rint(x * (127 / top)), scale = top / 127 with top = max |x| of the row, each operation in fp32.  d_q holds
+ * rows of nncf_int8_pitch(k) bytes (64 up to k = 64, else the next multiple of 128; zeros behind the k-th), 16-byte aligned.  A row of
+ * zeros has scale 0; a row with an infinity or NaN has zero codes and scale NaN.  normalize: the scale is that of the L2-normalised
+ * row (x * rsqrt(max(sum x^2, 1e-12)), model_framework.py:62-63).  k <= 131072. */
+int64_t nncf_int8_pitch(int32_t k);
+int nncf_quantize_rows(const void* d_x, int64_t x_stride, int32_t dtype, int64_t n, int32_t k, int32_t normalize, int8_t* d_q,
+                       float* d_scale, void* stream);
+/* d_out[n][k] = code * scale, 16-byte aligned. */
+int nncf_dequantize_rows(const int8_t* d_q, const float* d_scale, int64_t n, int32_t k, void* d_out, int32_t dtype, void* stream);
+/* d_out[i][j] = sx_i * st_j * sum_k qx_ik qt_jk + row_bias_i + col_bias_j (biases NULL or fp32), the integer sum exact; rows of
+ * d_out are out_stride elements of `dtype` apart, columns beyond c are not written. */
+int nncf_int8_scores(const int8_t* d_qx, const float* d_sx, int64_t m, const int8_t* d_qt, const float* d_st, int64_t c, int32_t k,
+                     const float* d_row_bias, const float* d_col_bias, void* d_out, int64_t out_stride, int32_t dtype, void* stream);
+
 /* Row movers and routing of the sharded path (no reference counterpart).
  * nncf_shard_route: for a batch's item ids d_cid[n], with item rows owned by rank id / item_shard:
  *   d_req[n_ranks][cap] = the unique ids to request from each owner (ascending, -1 padded) and

@@ -68,6 +68,13 @@ class TowerParams(ctypes.Structure):
         "conv_w", "conv_b", "bn1_gamma", "bn1_beta", "bn1_mean", "bn1_var", "item_spos", "item_start")]
 
 
+class Xent(ctypes.Structure):
+    """nncf_xent (include/nncf_hip.h): one call of the whole-catalogue softmax cross entropy."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("rows", "table", "target", "bias", "weight", "loss", "lse", "d_rows", "d_table", "d_bias")] +
+                [(n, ctypes.c_int64) for n in ("n", "c", "rows_stride", "table_stride")] +
+                [(n, ctypes.c_int32) for n in ("dim", "dtype", "reduction")] + [("scale", ctypes.c_float)])
+
+
 LOSS_CODES = {"skip-gram": 0, "mse": 1, "log-loss": 2, "max-margin": 3}
 
 
@@ -184,6 +191,10 @@ def _declare(lib):
         "nncf_group_sample_with_negs": [vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, u64, i32, i32, vp, vp, vp, vp, vp],
         "nncf_eval_topk": [vp, i64, i64, i32, vp, vp, i32, vp, vp, vp],
         "nncf_eval_whole": [vp, vp, i64, vp, i32, vp, vp, i32, vp, vp, vp],
+        "nncf_softmax_xent": [ctypes.POINTER(Xent), vp, i64, vp],
+        "nncf_quantize_rows": [vp, i64, i32, i64, i32, i32, vp, vp, vp],
+        "nncf_dequantize_rows": [vp, vp, i64, i32, vp, i32, vp],
+        "nncf_int8_scores": [vp, vp, i64, vp, vp, i64, i32, vp, vp, vp, i64, i32, vp],
         "nncf_plan_ids": [vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp],
     })
     for name, args in sig.items():
@@ -194,6 +205,10 @@ def _declare(lib):
     lib.nncf_tower_grad_floats.argtypes = [vp]
     lib.nncf_group_shuffle_ws_bytes.restype = i64
     lib.nncf_group_shuffle_ws_bytes.argtypes = [i64]
+    lib.nncf_softmax_xent_ws_bytes.restype = i64
+    lib.nncf_softmax_xent_ws_bytes.argtypes = [i64, i64, i32, i32, i32]
+    lib.nncf_int8_pitch.restype = i64
+    lib.nncf_int8_pitch.argtypes = [i32]
     lib.nncf_sampler_size.restype = i64
     lib.nncf_sampler_size.argtypes = [vp]
     lib.nncf_scatter_apply_ws_ints.restype = i64

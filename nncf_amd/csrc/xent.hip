@@ -1,0 +1,708 @@
+// Softmax cross entropy over the whole item table, with its gradients, without the logits.
+//
+//   z_ij = scale u_i . v_j + bias_j        loss_i = weight_i (log sum_j e^z_ij - z_i,t_i)
+//
+// One streaming kernel serves both directions.  It holds 32 OWN rows per wave (columns of the matrix instruction), walks over the
+// STREAM rows in tiles, and keeps per own row a a reference exponent M_a, l_a = sum_b 2^(y_ab - M_a) and O_a = sum_b 2^(y_ab - M_a)
+// x_b (y in base 2), so that n x c values are formed, used and dropped in registers:
+//   forward   own = users, stream = items, y = z log2(e):                     the normaliser and the mean item under p
+//   backward  own = items, stream = users, y = z log2(e) - lse + log2 |w|:    the columns of p times the user rows, exactly d_table
+// (the mean item is d_rows).  Logits are formed twice instead of being stored: 8 n c d operations where 6 are the least.
+//
+// The TARGET of a row is left out of the forward sums and joined in fp32: with A = log sum_{j != t} e^z_ij, loss = softplus(A - z_t)
+// and 1 - p_t = sigmoid(A - z_t) keep their relative accuracy as p_t -> 1, where 1 - p_t by subtraction keeps none; the gradient is
+// weight scale (1 - p_t) (mean_{j != t} v_j - v_t), and the backward pass takes -(1 - p_t) for the target's coefficient.
+//
+// Products of fp32 tables run on the f16 matrix pipe as two planes, x 2^b = hi + lo, with a power of two per ROW that brings its
+// largest value into [2^13, 2^14): hi + lo then hold 22 bits of every value within 2^16 of the row's largest and an absolute 2^-38 of
+// it below; three products (hi hi, hi lo, lo hi) leave about 6e-8 of sum |a b|, as an fp32 sum does.  No range of values is excluded
+// (the scale of a row of values below 2^-87 stops at 2^100).  The reference exponents M are whole numbers, so every rescaling is exact.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "common.h"
+#include "devutil.h"
+
+namespace nncf {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr int kOwn = 128;      // own rows of a workgroup: 4 waves x 32
+constexpr int kTile = 64;      // stream rows of a stage
+constexpr float kTop = 10.f;   // a new reference puts the largest exponent of a row at <= 2^10 ...
+constexpr float kRaise = 15.f; // ... and is taken again once one passes 2^15 (f16 ends at 2^16)
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct F16 {
+  typedef _Float16 E;
+  typedef f16x8 V;
+  static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+struct BF16 {
+  typedef __bf16 E;
+  typedef bf16x8 V;
+  static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// One side of the product, in the workspace.  img: [rows_pad][NP][DP] 16-bit values; inv = 2^-b (two planes only); h: what is added to
+// the exponent when the side streams; kq: the target coefficient of a user row; tgt: its target.
+struct Side {
+  const char* img;
+  const float* inv;
+  const float* h;
+  const float* kq;
+  const float* sgn;
+  const int32_t* tgt;
+  const float* bias;  // items
+  int64_t rows;       // rows of the call
+  int64_t rows_pad;   // a multiple of 128
+};
+struct Part {   // results of the streaming kernel: [splits][own rows_pad]
+  float *o, *m, *l;
+};
+
+// 16-byte chunks of a row are stored at chunk ^ g(row): a wave's ds_read_b128 of one chunk of 32 rows and its transposing
+// ds_read_b64 of 4 chunks of 4 consecutive rows then both meet every bank once.
+template <int NP, int DP>
+__device__ __forceinline__ int lds_at(int row, int plane, int chunk) {
+  if (DP == 128) {
+    const int g = ((row & 3) << 2) | ((row >> 2) & 3);
+    return row * (NP * 256) + plane * 256 + ((chunk ^ g) << 4);
+  } else {
+    const int u = (row >> 1) & 7, g = ((u & 1) << 2) | (u >> 1);
+    if (NP == 1) return row * 128 + ((chunk ^ g) << 4);
+    return row * 256 + ((plane ^ (row & 1)) << 7) + ((chunk ^ g) << 4);
+  }
+}
+
+template <class T, int NP, int DP>
+__device__ __forceinline__ typename T::V read_rows(const char* lds, int row, int plane, int chunk) {
+  return *reinterpret_cast<const typename T::V*>(lds + lds_at<NP, DP>(row, plane, chunk));
+}
+// column (32 dt + lane % 32) of rows r0 + 0..3 and r0 + 8 + 0..3, r0 = 16 s + 4 (lane / 32): the k order in which the accumulator
+// of the first product holds its rows, so that it is the second product's operand as it stands
+template <class T, int NP, int DP>
+__device__ __forceinline__ typename T::V read_cols(const char* lds, int plane, int base, int dt, int lane) {
+  typedef __attribute__((address_space(3))) s16x4_t* lp_t;
+  const int t = lane & 15, half = lane >> 5, sub = (lane >> 4) & 1;
+  const int row = base + 4 * half + (t >> 2), chunk = dt * 4 + sub * 2 + ((t & 3) >> 1), off = (t & 1) * 8;
+  const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp_t)(const_cast<char*>(lds) + lds_at<NP, DP>(row, plane, chunk) + off));
+  const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp_t)(const_cast<char*>(lds) + lds_at<NP, DP>(row + 8, plane, chunk) + off));
+  typedef short s16x8_t __attribute__((__vector_size__(8 * sizeof(short))));
+  const s16x8_t c = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(typename T::V, c);
+}
+
+// The streaming kernel.  BWD: own rows are items.  WT: row weights of either sign.  MEAN: the O sums are wanted.
+template <class T, int NP, int DP, bool BWD, bool WT, bool MEAN>
+__global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str, Part part, float scale2, int tiles, int tiles_per_split) {
+  typedef typename T::V V;
+  constexpr int kRow = NP * DP * 2;             // bytes of an image row
+  constexpr int KS = DP / 16, DT = DP / 32;
+  __shared__ __attribute__((aligned(16))) char s_img[kTile * kRow];
+  __shared__ __attribute__((aligned(16))) float s_inv[kTile], s_h[kTile], s_sgn[kTile];
+  __shared__ __attribute__((aligned(16))) int32_t s_tgt[kTile];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int split = blockIdx.x;
+  const int64_t own0 = (int64_t)blockIdx.y * kOwn + wave * 32, own_row = own0 + col;
+
+  V of[NP][KS];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      of[p][k] = *reinterpret_cast<const V*>(own.img + own_row * kRow + p * (DP * 2) + (2 * k + half) * 16);
+  const float c = NP == 2 ? scale2 * own.inv[own_row] : scale2;
+  const bool inside = own_row < own.rows;
+  const int32_t own_tgt = !BWD && inside ? own.tgt[own_row] : -1;
+  const float add = BWD && inside && own.bias ? own.bias[own_row] * kLog2e : 0.f;
+
+  f32x16 o[MEAN ? DT : 1];
+#pragma unroll
+  for (int d = 0; d < (MEAN ? DT : 1); ++d) o[d] = 0.f;
+  float m = 0.f, l = 0.f;
+  bool seen = false;
+
+  const int t0 = split * tiles_per_split, t1 = min(tiles, t0 + tiles_per_split);
+  for (int tile = t0; tile < t1; ++tile) {
+    const int64_t row0 = (int64_t)tile * kTile;
+    __syncthreads();
+    for (int i = tid; i < kTile * kRow / 16; i += 256) {
+      const int row = i / (kRow / 16), in = i % (kRow / 16), p = in / (DP / 8), chunk = in % (DP / 8);
+      *reinterpret_cast<float4*>(s_img + lds_at<NP, DP>(row, p, chunk)) =
+          *reinterpret_cast<const float4*>(str.img + (row0 + row) * kRow + in * 16);
+    }
+    if (tid < kTile) {
+      s_h[tid] = str.h[row0 + tid];
+      if (NP == 2) s_inv[tid] = str.inv[row0 + tid];
+      if (WT) s_sgn[tid] = str.sgn[row0 + tid];
+      if (BWD) s_tgt[tid] = row0 + tid < str.rows ? str.tgt[row0 + tid] : -1;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int r = 0; r < kTile / 32; ++r) {
+      f32x16 s = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const V a = read_rows<T, NP, DP>(s_img, 32 * r + col, 0, 2 * k + half);
+        s = T::mfma(a, of[0][k], s);
+        if (NP == 2) {
+          const V b = read_rows<T, NP, DP>(s_img, 32 * r + col, 1, 2 * k + half);
+          s = T::mfma(a, of[NP - 1][k], s);
+          s = T::mfma(b, of[0][k], s);
+        }
+      }
+      float d[16], iv[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = 32 * r + 8 * g + 4 * half;
+        const float4 h4 = *reinterpret_cast<const float4*>(s_h + at);
+        const float hv[4] = {h4.x, h4.y, h4.z, h4.w};
+        float4 i4 = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (NP == 2) i4 = *reinterpret_cast<const float4*>(s_inv + at);
+        const float ivv[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          iv[4 * g + e] = ivv[e];
+          d[4 * g + e] = fmaf(NP == 2 ? s[4 * g + e] * ivv[e] : s[4 * g + e], c, hv[e] - (m - add));
+        }
+      }
+      // targets: a wave-uniform branch, taken by one sub-tile in c / 32 per own row
+      uint32_t hit = 0;
+      if (!BWD) {
+        if (__any((uint32_t)(own_tgt - (int32_t)(row0 + 32 * r)) < 32u)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if ((int32_t)(row0 + 32 * r) + 8 * (i >> 2) + 4 * half + (i & 3) == own_tgt) d[i] = -INFINITY;
+        }
+      } else {
+        const uint32_t in = (uint32_t)(s_tgt[32 * r + col] - (int32_t)own0);
+        if (__any(in < 32u)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = 32 * r + 8 * (i >> 2) + 4 * half + (i & 3);
+            if (s_tgt[at] == (int32_t)own_row) {
+              hit |= 1u << i;
+              d[i] = __builtin_amdgcn_logf(fabsf(str.kq[row0 + at])) - m;
+            }
+          }
+        }
+      }
+      float top = d[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, d[i]);
+      if (__any(top > kRaise || (!seen && top > -INFINITY))) {
+        top = fmaxf(top, __shfl_xor(top, 32));   // both halves of a column keep one reference
+        const bool move = top > kRaise || (!seen && top > -INFINITY);
+        const float by = move ? ceilf(top) - kTop : 0.f;
+        const float f = seen ? __builtin_amdgcn_exp2f(-by) : 1.f;
+        seen = seen || move;
+        m += by;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] -= by;
+        if (MEAN) {
+#pragma unroll
+          for (int t = 0; t < DT; ++t) o[t] *= f;
+        }
+      }
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(d[i]);
+      if (WT) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 w4 = *reinterpret_cast<const float4*>(s_sgn + 32 * r + 8 * g + 4 * half);
+          p[4 * g] *= w4.x;
+          p[4 * g + 1] *= w4.y;
+          p[4 * g + 2] *= w4.z;
+          p[4 * g + 3] *= w4.w;
+        }
+      }
+      float plo[16];
+      if (BWD && NP == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) plo[i] = 0.f;
+      }
+      const bool any_hit = BWD && __any(hit != 0);
+      if (any_hit) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (hit >> i & 1) {
+            p[i] = -ldexpf(str.kq[row0 + 32 * r + 8 * (i >> 2) + 4 * half + (i & 3)], (int)-m);
+            if (NP == 1) plo[i] = p[i] - (float)(typename T::E)p[i];
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        // 2^b = 1 / 2^-b, by its exponent
+        const float up = NP == 2 ? __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, iv[i])) : 1.f;
+        l = fmaf(p[i], up, l);
+      }
+      if (MEAN) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          V hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            hi[e] = (typename T::E)p[8 * q + e];
+            if (NP == 2) lo[e] = (typename T::E)(p[8 * q + e] - (float)hi[e]);
+          }
+#pragma unroll
+          for (int t = 0; t < DT; ++t) {
+            const V a = read_cols<T, NP, DP>(s_img, 0, 32 * r + 16 * q, t, lane);
+            o[t] = T::mfma(a, hi, o[t]);
+            if (NP == 2) {
+              const V b = read_cols<T, NP, DP>(s_img, NP - 1, 32 * r + 16 * q, t, lane);
+              o[t] = T::mfma(a, lo, o[t]);
+              o[t] = T::mfma(b, hi, o[t]);
+            }
+          }
+          if (NP == 1 && any_hit) {   // one plane: what rounding took from a target's coefficient, the largest terms of its sum
+#pragma unroll
+            for (int e = 0; e < 8; ++e) lo[e] = (typename T::E)plo[8 * q + e];
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] = T::mfma(read_cols<T, NP, DP>(s_img, 0, 32 * r + 16 * q, t, lane), lo, o[t]);
+          }
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 32);
+  const int64_t at = (int64_t)split * own.rows_pad + own_row;
+  if (half == 0) {
+    part.m[at] = seen ? m : -INFINITY;
+    part.l[at] = l;
+  }
+  if (MEAN) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(part.o + at * DP + 32 * t + 8 * g + 4 * half) =
+            make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
+  }
+}
+
+// ---- images ------------------------------------------------------------------------------------------------------------------
+template <class E>
+__device__ __forceinline__ void load8(const E* row, int c0, int d, bool vec, float* x) {
+  if (vec) {   // rows start on a multiple of 4 elements
+    typedef E E4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int at = c0 + 4 * q;
+      if (at + 4 <= d) {
+        const E4 v = *reinterpret_cast<const E4*>(row + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * q + e] = (float)v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * q + e] = at + e < d ? (float)row[at + e] : 0.f;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = c0 + e < d ? (float)row[c0 + e] : 0.f;
+  }
+}
+
+struct PrepSide {
+  const void* src;
+  int64_t stride, rows, rows_pad;
+  const int32_t* keep;    // users: rows with keep < 0 are not used
+  const float* bias;      // items: rows at -inf are not used
+  char* img;
+  float *inv, *h, *sgn;
+  int vec;
+};
+
+// One row per DP / 8 lanes (8 columns each): the row in one or two 16-bit planes, its scale, and for an item what streams with it.
+template <class E, int NP, int DP>
+__global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, int64_t a_blocks, int d, int32_t* valid, int n) {
+  constexpr int LR = DP / 8;
+  if (blockIdx.x == gridDim.x - 1) {   // rows that have a target, by one workgroup
+    __shared__ int s_cnt[4];
+    int cnt = 0;
+    for (int i = threadIdx.x; i < n; i += 256) cnt += a.keep[i] >= 0;
+    cnt = wave_sum_i(cnt);
+    if ((threadIdx.x & 63) == 0) s_cnt[threadIdx.x >> 6] = cnt;
+    __syncthreads();
+    if (threadIdx.x == 0) *valid = s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3];
+    return;
+  }
+  const bool first = (int64_t)blockIdx.x < a_blocks;
+  const PrepSide s = first ? a : b;
+  const int64_t row = ((int64_t)blockIdx.x - (first ? 0 : a_blocks)) * (256 / LR) + threadIdx.x / LR;
+  if (row >= s.rows_pad) return;
+  const int q = threadIdx.x % LR;
+  bool use = row < s.rows;
+  float bias = 0.f;
+  if (use && s.keep) use = s.keep[row] >= 0;
+  if (use && s.bias) {
+    bias = s.bias[row];
+    use = !(bias == -INFINITY);
+  }
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  if (use) load8(reinterpret_cast<const E*>(s.src) + row * s.stride, 8 * q, d, s.vec != 0, x);
+  float inv = 1.f, shift = 0.f;
+  char* out = s.img + row * (NP * DP * 2) + q * 16;
+  if constexpr (NP == 2) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+    for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    int b = 0;
+    if (top > 0.f && top < INFINITY) b = min(100, 14 - __builtin_amdgcn_frexp_expf(top));
+    inv = ldexpf(1.f, -b);
+    shift = (float)b;
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = ldexpf(x[e], b);
+      hi[e] = (_Float16)v;
+      lo[e] = (_Float16)(v - (float)hi[e]);
+    }
+    *reinterpret_cast<f16x8*>(out) = hi;
+    *reinterpret_cast<f16x8*>(out + DP * 2) = lo;
+  } else {
+    typedef E E8 __attribute__((ext_vector_type(8)));
+    E8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (E)x[e];
+    *reinterpret_cast<E8*>(out) = v;
+  }
+  if (q == 0) {
+    if (NP == 2) s.inv[row] = inv;
+    if (s.sgn) s.sgn[row] = 1.f;
+    s.h[row] = use && !s.keep ? bias * kLog2e - shift : -INFINITY;   // users: written once their normaliser is known
+  }
+}
+
+// ---- joining the splits ------------------------------------------------------------------------------------------------------
+struct RowsOut {
+  const void *rows, *table;
+  int64_t rows_stride, table_stride;
+  const float *bias, *weight;
+  const int32_t *target, *valid;
+  float *loss_rows, *lse, *h, *kq, *sgn;
+  const float* inv;
+  void* d_rows;
+  float scale;
+  int64_t n, c, rows_pad;
+  int d, mean, splits;
+};
+
+// One wave per row: joins its splits, adds the target, writes loss, lse, d_rows and what the row streams with in the backward pass.
+template <class E, int NP, int DP, bool MEAN>
+__global__ void __launch_bounds__(256) xent_rows_kernel(RowsOut a, Part part) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.n) return;
+  const int32_t t = a.target[row];
+  const bool has = t >= 0, bad = has && t >= a.c;
+  const E* u = reinterpret_cast<const E*>(a.rows) + row * a.rows_stride;
+  const E* v = reinterpret_cast<const E*>(a.table) + (int64_t)(has && !bad ? t : 0) * a.table_stride;
+  float top = -INFINITY;
+  for (int k = lane; k < a.splits; k += 64) top = fmaxf(top, part.m[(int64_t)k * a.rows_pad + row]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  const bool some = top > -INFINITY;
+  if (has && some) {
+    for (int k = lane; k < a.splits; k += 64) {
+      const int64_t at = (int64_t)k * a.rows_pad + row;
+      const float mk = part.m[at];
+      if (mk > -INFINITY) l += part.l[at] * __builtin_amdgcn_exp2f(mk - top);
+    }
+    l = wave_sum(l);
+    if (MEAN) {
+#pragma unroll 4
+      for (int k = 0; k < a.splits; ++k) {
+        const int64_t at = (int64_t)k * a.rows_pad + row;
+        const float mk = part.m[at], f = mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - top) : 0.f;
+        o0 = fmaf(part.o[at * DP + lane], f, o0);
+        if (DP == 128) o1 = fmaf(part.o[at * DP + 64 + lane], f, o1);
+      }
+    }
+  }
+  float u0 = 0.f, u1 = 0.f, v0 = 0.f, v1 = 0.f;
+  const float beta = has && !bad && a.bias ? a.bias[t] : 0.f;
+  const bool out = beta == -INFINITY;     // the target itself is left out: nothing to learn from
+  if (has && !bad && !out) {
+    if (lane < a.d) { u0 = (float)u[lane]; v0 = (float)v[lane]; }
+    if (lane + 64 < a.d) { u1 = (float)u[lane + 64]; v1 = (float)v[lane + 64]; }
+  }
+  const float zt = out ? -INFINITY : fmaf(a.scale, wave_sum(fmaf(u1, v1, u0 * v0)), beta);
+  const float rest = some && !(l == 0.f) ? (top + log2f(l)) * kLn2 : -INFINITY;   // log sum over the other items
+  const float apart = rest - zt;
+  float each, q, lse;
+  if (out) {
+    each = INFINITY;
+    q = 0.f;
+    lse = rest;
+  } else {
+    const float e = expf(-fabsf(apart));                 // rest = -inf: 0
+    each = fmaxf(apart, 0.f) + log1pf(e);
+    q = apart >= 0.f ? 1.f / (1.f + e) : e / (1.f + e);
+    lse = fmaxf(rest, zt) + log1pf(e);
+  }
+  float w = a.weight ? a.weight[row] : 1.f;
+  if (bad) {
+    each = lse = q = NAN;
+  }
+  if (!has) {
+    each = lse = q = w = 0.f;
+  }
+  const float g = a.mean ? w / (float)max(1, *a.valid) : w;
+  if (lane == 0) {
+    // a weight of zero takes the row out of the loss, whatever its loss is
+    a.loss_rows[row] = has && !(w == 0.f) ? w * each : 0.f;
+    a.lse[row] = lse;
+    const float inv = NP == 2 ? a.inv[row] : 1.f;
+    if (a.h) {
+      const bool dead = !has || out || w == 0.f;
+      const float shift = NP == 2 ? (float)(__builtin_amdgcn_frexp_expf(inv) - 1) : 0.f;   // log2 of the power of two
+      a.h[row] = dead ? -INFINITY : (__builtin_amdgcn_logf(fabsf(w)) - lse * kLog2e) + shift;
+      a.kq[row] = dead ? 0.f : w * q * inv;
+      a.sgn[row] = w < 0.f ? -1.f : 1.f;
+    }
+  }
+  if (MEAN) {
+    const float k = w == 0.f ? 0.f : a.scale * g * q;
+    const bool zero = !has || out || w == 0.f || q == 0.f;
+    const float r = l == 0.f ? 0.f : 1.f / l;
+    E* dr = reinterpret_cast<E*>(a.d_rows) + row * a.d;
+    if (lane < a.d) dr[lane] = (E)(zero ? 0.f : k * fmaf(o0, r, -v0));
+    if (lane + 64 < a.d) dr[lane + 64] = (E)(zero ? 0.f : k * fmaf(o1, r, -v1));
+  }
+}
+
+struct TableOut {
+  const float* bias;
+  const int32_t* valid;
+  const float* loss_rows;
+  float* loss;
+  void* d_table;
+  float* d_bias;
+  float scale;
+  int64_t n, c, rows_pad;
+  int d, mean, splits, reduce;
+};
+
+// sum of the rows' losses, in row order per lane: one workgroup
+__device__ __forceinline__ void total_loss(const float* rows, int64_t n, int mean, const int32_t* valid, float* out) {
+  __shared__ double s_sum[4];
+  double sum = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 256) sum += (double)rows[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    *out = (float)(mean ? all / (double)max(1, *valid) : all);
+  }
+}
+
+__global__ void __launch_bounds__(256) xent_loss_kernel(TableOut a) { total_loss(a.loss_rows, a.n, a.mean, a.valid, a.loss); }
+
+// One row of the table per DP / 4 lanes: joins its splits, applies the scales; the last workgroup sums the losses.
+template <class E, int DP>
+__global__ void __launch_bounds__(256) xent_table_kernel(TableOut a, Part part) {
+  if (a.reduce && blockIdx.x == gridDim.x - 1) {
+    total_loss(a.loss_rows, a.n, a.mean, a.valid, a.loss);
+    return;
+  }
+  constexpr int LR = DP / 4;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+  const int q = threadIdx.x % LR;
+  if (row >= a.c) return;
+  const bool out = a.bias && a.bias[row] == -INFINITY;
+  float top = -INFINITY;
+  for (int k = 0; k < a.splits; ++k) top = fmaxf(top, part.m[(int64_t)k * a.rows_pad + row]);
+  float l = 0.f;
+  float4 o = zero4();
+  if (top > -INFINITY && !out) {
+#pragma unroll 4
+    for (int k = 0; k < a.splits; ++k) {
+      const int64_t at = (int64_t)k * a.rows_pad + row;
+      const float mk = part.m[at], f = mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - top) : 0.f;
+      l = fmaf(part.l[at], f, l);
+      o = fma4(f, *reinterpret_cast<const float4*>(part.o + at * DP + 4 * q), o);
+    }
+    const float share = a.mean ? 1.f / (float)max(1, *a.valid) : 1.f;
+    l = ldexpf(l, (int)top) * share;
+    const float k = a.scale * share;
+    o.x = ldexpf(o.x, (int)top) * k;
+    o.y = ldexpf(o.y, (int)top) * k;
+    o.z = ldexpf(o.z, (int)top) * k;
+    o.w = ldexpf(o.w, (int)top) * k;
+  }
+  const float v[4] = {o.x, o.y, o.z, o.w};
+  E* dst = reinterpret_cast<E*>(a.d_table) + row * a.d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (4 * q + e < a.d) dst[4 * q + e] = (E)v[e];
+  if (q == 0 && a.d_bias) a.d_bias[row] = l;
+}
+// ---- host --------------------------------------------------------------------------------------------------------------------
+inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+// Splits of the stream axis: enough workgroups for two on every CU, at least two stages each; a multiple of 8 where there are as
+// many, so that the workgroups of one XCD (consecutive ids go round the eight of them) walk over the same part of the stream.
+inline int splits_for(int64_t own_tiles, int64_t stream_tiles) {
+  int64_t s = up(512, own_tiles) / own_tiles;
+  s = std::min(s, std::max<int64_t>(1, stream_tiles / 2));
+  if (s > 8) s = s / 8 * 8;
+  return (int)std::min<int64_t>(s, 256);
+}
+
+struct Layout {
+  int np, dp;
+  int64_t npad, cpad;
+  int fs, bs;                       // splits of the two passes
+  int64_t u_img, u_inv, u_h, u_kq, u_sgn, v_img, v_inv, v_h, o, m, l, loss, valid, bytes;
+};
+
+Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
+  Layout y{};
+  y.np = dtype == NNCF_F32 ? 2 : 1;
+  y.dp = d <= 64 ? 64 : 128;
+  y.npad = up(n, kOwn);
+  y.cpad = up(c, kOwn);
+  y.fs = splits_for(y.npad / kOwn, up(c, kTile) / kTile);
+  y.bs = splits_for(y.cpad / kOwn, up(n, kTile) / kTile);
+  int64_t at = 0;
+  auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };
+  const int64_t row = (int64_t)y.np * y.dp * 2;
+  const int64_t part = std::max((int64_t)y.fs * y.npad, grad ? (int64_t)y.bs * y.cpad : 0);
+  y.u_img = take(y.npad * row);
+  y.u_inv = take(y.npad * 4);
+  y.u_h = take(y.npad * 4);
+  y.u_kq = take(y.npad * 4);
+  y.u_sgn = take(y.npad * 4);
+  y.v_img = take(y.cpad * row);
+  y.v_inv = take(y.cpad * 4);
+  y.v_h = take(y.cpad * 4);
+  y.o = take(grad ? part * y.dp * 4 : 0);
+  y.m = take(part * 4);
+  y.l = take(part * 4);
+  y.loss = take(n * 4);
+  y.valid = take(4);
+  y.bytes = at;
+  return y;
+}
+
+template <class T, int NP, int DP>
+int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
+  typedef typename std::conditional<NP == 2, float, typename T::E>::type E;
+  const bool grad = x->d_rows != nullptr;
+  auto f = [ws](int64_t at) { return reinterpret_cast<float*>(ws + at); };
+  int32_t* valid = reinterpret_cast<int32_t*>(ws + y.valid);
+  auto vec = [](const void* p, int64_t stride) { return ((uintptr_t)p % (4 * sizeof(E)) == 0 && stride % 4 == 0) ? 1 : 0; };
+  const PrepSide pu{x->rows, x->rows_stride, x->n, y.npad, x->target, nullptr, ws + y.u_img, f(y.u_inv), f(y.u_h), f(y.u_sgn),
+                    vec(x->rows, x->rows_stride)};
+  const PrepSide pv{x->table, x->table_stride, x->c, y.cpad, nullptr, x->bias, ws + y.v_img, f(y.v_inv), f(y.v_h), nullptr,
+                    vec(x->table, x->table_stride)};
+  constexpr int kPrepRows = 256 / (DP / 8);
+  const int64_t ub = up(y.npad, kPrepRows) / kPrepRows, vb = up(y.cpad, kPrepRows) / kPrepRows;
+  {
+    ProfScope ps("xent_prep_kernel", st);
+    hipLaunchKernelGGL((xent_prep_kernel<E, NP, DP>), dim3((unsigned)(ub + vb + 1)), dim3(256), 0, st, pu, pv, ub, x->dim, valid,
+                       (int)x->n);
+  }
+  const Side u{ws + y.u_img, f(y.u_inv), f(y.u_h), f(y.u_kq), f(y.u_sgn), x->target, nullptr, x->n, y.npad};
+  const Side v{ws + y.v_img, f(y.v_inv), f(y.v_h), nullptr, nullptr, nullptr, x->bias, x->c, y.cpad};
+  const Part part{f(y.o), f(y.m), f(y.l)};
+  const float scale2 = x->scale * kLog2e;
+  {
+    const int tiles = (int)(up(x->c, kTile) / kTile), per = (tiles + y.fs - 1) / y.fs;
+    const dim3 grid((unsigned)y.fs, (unsigned)(y.npad / kOwn));
+    ProfScope ps("xent_stream_kernel", st);
+    if (grad)
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, true>), grid, dim3(256), 0, st, u, v, part, scale2, tiles, per);
+    else
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, false>), grid, dim3(256), 0, st, u, v, part, scale2, tiles, per);
+  }
+  const bool scalar = x->reduction != NNCF_NONE;
+  const int mean = x->reduction == NNCF_MEAN;
+  float* loss_rows = scalar ? f(y.loss) : x->loss;
+  const RowsOut ro{x->rows, x->table, x->rows_stride, x->table_stride, x->bias, x->weight, x->target, valid, loss_rows, x->lse,
+                   grad ? f(y.u_h) : nullptr, f(y.u_kq), f(y.u_sgn), f(y.u_inv), x->d_rows, x->scale, x->n, x->c, y.npad, x->dim, mean, y.fs};
+  {
+    ProfScope ps("xent_rows_kernel", st);
+    const dim3 grid((unsigned)((x->n + 3) / 4));
+    if (grad)
+      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, true>), grid, dim3(256), 0, st, ro, part);
+    else
+      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, false>), grid, dim3(256), 0, st, ro, part);
+  }
+  TableOut to{x->bias, valid, loss_rows, x->loss, x->d_table, x->d_bias, x->scale, x->n, x->c, y.cpad, x->dim, mean, y.bs, scalar};
+  if (!grad) {
+    if (scalar) hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, st, to);
+  } else {
+    const int tiles = (int)(up(x->n, kTile) / kTile), per = (tiles + y.bs - 1) / y.bs;
+    const dim3 grid((unsigned)y.bs, (unsigned)(y.cpad / kOwn));
+    {
+      ProfScope ps("xent_stream_kernel", st);
+      if (x->weight)
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, true, true>), grid, dim3(256), 0, st, v, u, part, scale2, tiles, per);
+      else
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, false, true>), grid, dim3(256), 0, st, v, u, part, scale2, tiles, per);
+    }
+    ProfScope ps("xent_table_kernel", st);
+    constexpr int kRows = 256 / (DP / 4);
+    hipLaunchKernelGGL((xent_table_kernel<E, DP>), dim3((unsigned)((x->c + kRows - 1) / kRows + (scalar ? 1 : 0))), dim3(256), 0, st, to, part);
+  }
+  NNCF_HIP_CHECK(hipGetLastError());
+  return NNCF_OK;
+}
+
+int check_shape(int64_t n, int64_t c, int32_t dim, int32_t dtype) {
+  NNCF_REQUIRE(n > 0 && n <= (int64_t)kOwn * 65535, "n = %lld rows out of range (1..%lld)", (long long)n, (long long)kOwn * 65535);
+  // own tiles of a launch are its grid's second dimension
+  NNCF_REQUIRE(c > 0 && c <= (int64_t)kOwn * 65535, "c = %lld items out of range (1..%lld)", (long long)c, (long long)kOwn * 65535);
+  NNCF_REQUIRE(dim > 0 && dim <= 128, "dim = %d out of range (1..128)", dim);
+  NNCF_REQUIRE(dtype == NNCF_F32 || dtype == NNCF_F16 || dtype == NNCF_BF16, "dtype = %d unknown", dtype);
+  return NNCF_OK;
+}
+}  // namespace
+}  // namespace nncf
+
+extern "C" int64_t nncf_softmax_xent_ws_bytes(int64_t n, int64_t c, int32_t dim, int32_t dtype, int32_t with_grad) {
+  if (nncf::check_shape(n, c, dim, dtype) != NNCF_OK) return -1;
+  return nncf::layout(n, c, dim, dtype, with_grad != 0).bytes;
+}
+
+extern "C" int nncf_softmax_xent(const nncf_xent* x, void* d_ws, int64_t ws_bytes, void* stream) {
+  using namespace nncf;
+  NNCF_REQUIRE(x != nullptr, "NULL argument");
+  const int rc = check_shape(x->n, x->c, x->dim, x->dtype);
+  if (rc) return rc;
+  NNCF_REQUIRE(x->rows && x->table && x->target && x->loss && x->lse && d_ws, "NULL argument");
+  NNCF_REQUIRE((x->d_rows != nullptr) == (x->d_table != nullptr), "d_rows and d_table are computed together");
+  NNCF_REQUIRE(!x->d_bias || (x->bias && x->d_rows), "d_bias needs a bias and the other gradients");
+  NNCF_REQUIRE(x->rows_stride >= x->dim && x->table_stride >= x->dim, "a row stride is below dim = %d", x->dim);
+  NNCF_REQUIRE(x->reduction == NNCF_NONE || x->reduction == NNCF_MEAN || x->reduction == NNCF_SUM, "reduction = %d unknown", x->reduction);
+  NNCF_REQUIRE(std::isfinite(x->scale), "scale must be finite");
+  const uintptr_t es = x->dtype == NNCF_F32 ? 4 : 2;
+  NNCF_REQUIRE((uintptr_t)x->rows % es == 0 && (uintptr_t)x->table % es == 0 && (uintptr_t)x->d_rows % es == 0 &&
+               (uintptr_t)x->d_table % es == 0, "a tensor is not aligned to its elements");
+  const Layout y = layout(x->n, x->c, x->dim, x->dtype, x->d_rows != nullptr);
+  NNCF_REQUIRE(ws_bytes >= y.bytes, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)y.bytes);
+  NNCF_REQUIRE(((uintptr_t)d_ws & 255) == 0, "workspace must be 256-byte aligned");
+  char* ws = reinterpret_cast<char*>(d_ws);
+  hipStream_t st = as_stream(stream);
+  const bool wide = y.dp == 128;
+  if (x->dtype == NNCF_F32) return wide ? run<F16, 2, 128>(x, y, ws, st) : run<F16, 2, 64>(x, y, ws, st);
+  if (x->dtype == NNCF_F16) return wide ? run<F16, 1, 128>(x, y, ws, st) : run<F16, 1, 64>(x, y, ws, st);
+  return wide ? run<BF16, 1, 128>(x, y, ws, st) : run<BF16, 1, 64>(x, y, ws, st);
+}
