@@ -79,6 +79,63 @@ __device__ __forceinline__ int lds_at(int row, int plane, int chunk) {
   }
 }
 
+// the inverse: byte offset in a tile of the row-major image of what lies in 16-byte slot i of its LDS form
+template <int NP, int DP>
+__device__ __forceinline__ int image_at(int i) {
+  if (DP == 128) {
+    const int row = i / (NP * 16), g = ((row & 3) << 2) | ((row >> 2) & 3);
+    return (i & ~15) * 16 + (((i & 15) ^ g) << 4);
+  } else {
+    const int row = i / (NP * 8), u = (row >> 1) & 7, g = ((u & 1) << 2) | (u >> 1);
+    const int plane = NP == 1 ? 0 : (i >> 3 & 1) ^ (row & 1);
+    return row * (NP * 128) + plane * 128 + (((i & 7) ^ g) << 4);
+  }
+}
+
+// A stage of stream rows in LDS, and its asynchronous filling: global memory to LDS without a register, 1 KB per wave and instruction.
+template <int NP, int DP>
+struct __attribute__((aligned(16))) Stage {
+  char img[kTile * NP * DP * 2];
+  float h[kTile], inv[kTile], sgn[kTile];
+  int32_t tgt[kTile];
+};
+typedef const __attribute__((address_space(1))) void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+// The slots a wave fills lie a multiple of 16 rows apart, where the order of chunks is the same: one lane offset (two for rows of 512
+// bytes) serves them all.
+template <int NP, int DP>
+struct Filler {
+  static constexpr int kRow = NP * DP * 2, kEach = kTile * kRow / 16 / 256, kOff = kRow == 512 ? 2 : 1;
+  int off[kOff];
+  static __device__ __forceinline__ int slot(int j, int wave) {   // in units of 64 slots
+    return kOff == 2 ? (j & 1) + 2 * wave + 8 * (j >> 1) : wave + 4 * j;
+  }
+  __device__ __forceinline__ Filler(int wave, int lane) {
+#pragma unroll
+    for (int j = 0; j < kOff; ++j) off[j] = image_at<NP, DP>(slot(j, wave) * 64 + lane);
+  }
+};
+
+template <int NP, int DP, bool BWD, bool WT>
+__device__ __forceinline__ void fill(Stage<NP, DP>& to, const Filler<NP, DP>& f, const Side& str, int64_t row0, int wave, int lane) {
+  typedef Filler<NP, DP> F;
+#pragma unroll
+  for (int j = 0; j < F::kEach; ++j) {
+    constexpr int step = F::kOff == 2 ? 16 * F::kRow : 4096;     // bytes of the image between a wave's equal offsets
+    const char* src = str.img + row0 * F::kRow + (j / F::kOff) * step;
+    __builtin_amdgcn_global_load_lds((gptr_t)(src + f.off[j % F::kOff]), (lptr_t)(to.img + F::slot(j, wave) * 1024), 16, 0, 0);
+  }
+  if (wave == 0) __builtin_amdgcn_global_load_lds((gptr_t)(str.h + row0 + lane), (lptr_t)to.h, 4, 0, 0);
+  if (NP == 2 && wave == 1) __builtin_amdgcn_global_load_lds((gptr_t)(str.inv + row0 + lane), (lptr_t)to.inv, 4, 0, 0);
+  if (WT && wave == 2) __builtin_amdgcn_global_load_lds((gptr_t)(str.sgn + row0 + lane), (lptr_t)to.sgn, 4, 0, 0);
+  if (BWD && wave == 3) __builtin_amdgcn_global_load_lds((gptr_t)(str.tgt + row0 + lane), (lptr_t)to.tgt, 4, 0, 0);
+}
+__device__ __forceinline__ void filled() {   // this wave's part has arrived, and everyone's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 template <class T, int NP, int DP>
 __device__ __forceinline__ typename T::V read_rows(const char* lds, int row, int plane, int chunk) {
   return *reinterpret_cast<const typename T::V*>(lds + lds_at<NP, DP>(row, plane, chunk));
@@ -103,10 +160,8 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
   typedef typename T::V V;
   constexpr int kRow = NP * DP * 2;             // bytes of an image row
   constexpr int KS = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) char s_img[kTile * kRow];
-  __shared__ __attribute__((aligned(16))) float s_inv[kTile], s_h[kTile], s_sgn[kTile];
-  __shared__ __attribute__((aligned(16))) int32_t s_tgt[kTile];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  __shared__ Stage<NP, DP> s_a, s_b;            // two objects, so that a read of one does not wait for the filling of the other
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int split = blockIdx.x;
   const int64_t own0 = (int64_t)blockIdx.y * kOwn + wave * 32, own_row = own0 + col;
 
@@ -118,7 +173,8 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
       of[p][k] = *reinterpret_cast<const V*>(own.img + own_row * kRow + p * (DP * 2) + (2 * k + half) * 16);
   const float c = NP == 2 ? scale2 * own.inv[own_row] : scale2;
   const bool inside = own_row < own.rows;
-  const int32_t own_tgt = !BWD && inside ? own.tgt[own_row] : -1;
+  const int32_t own_id = (int32_t)own_row;
+  const int32_t own_tgt = BWD ? -1 : own.tgt[own_row];
   const float add = BWD && inside && own.bias ? own.bias[own_row] * kLog2e : 0.f;
 
   f32x16 o[MEAN ? DT : 1];
@@ -128,21 +184,10 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
   bool seen = false;
 
   const int t0 = split * tiles_per_split, t1 = min(tiles, t0 + tiles_per_split);
-  for (int tile = t0; tile < t1; ++tile) {
-    const int64_t row0 = (int64_t)tile * kTile;
-    __syncthreads();
-    for (int i = tid; i < kTile * kRow / 16; i += 256) {
-      const int row = i / (kRow / 16), in = i % (kRow / 16), p = in / (DP / 8), chunk = in % (DP / 8);
-      *reinterpret_cast<float4*>(s_img + lds_at<NP, DP>(row, p, chunk)) =
-          *reinterpret_cast<const float4*>(str.img + (row0 + row) * kRow + in * 16);
-    }
-    if (tid < kTile) {
-      s_h[tid] = str.h[row0 + tid];
-      if (NP == 2) s_inv[tid] = str.inv[row0 + tid];
-      if (WT) s_sgn[tid] = str.sgn[row0 + tid];
-      if (BWD) s_tgt[tid] = row0 + tid < str.rows ? str.tgt[row0 + tid] : -1;
-    }
-    __syncthreads();
+  auto work = [&](const Stage<NP, DP>& st, int64_t row0) __attribute__((always_inline)) {
+    const char* s_img = st.img;
+    const float *s_h = st.h, *s_inv = st.inv, *s_sgn = st.sgn;
+    const int32_t* s_tgt = st.tgt;
 #pragma unroll 1
     for (int r = 0; r < kTile / 32; ++r) {
       f32x16 s = 0.f;
@@ -185,7 +230,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int at = 32 * r + 8 * (i >> 2) + 4 * half + (i & 3);
-            if (s_tgt[at] == (int32_t)own_row) {
+            if (s_tgt[at] == own_id) {
               hit |= 1u << i;
               d[i] = __builtin_amdgcn_logf(fabsf(str.kq[row0 + at])) - m;
             }
@@ -271,6 +316,20 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
         }
       }
     }
+  };
+  const Filler<NP, DP> filler(wave, lane);
+  if (t0 < t1) {
+    fill<NP, DP, BWD, WT>(s_a, filler, str, (int64_t)t0 * kTile, wave, lane);
+    filled();
+    for (int tile = t0; tile < t1; tile += 2) {
+      if (tile + 1 < t1) fill<NP, DP, BWD, WT>(s_b, filler, str, (int64_t)(tile + 1) * kTile, wave, lane);
+      work(s_a, (int64_t)tile * kTile);
+      filled();
+      if (tile + 1 >= t1) break;
+      if (tile + 2 < t1) fill<NP, DP, BWD, WT>(s_a, filler, str, (int64_t)(tile + 2) * kTile, wave, lane);
+      work(s_b, (int64_t)(tile + 1) * kTile);
+      filled();
+    }
   }
   l += __shfl_xor(l, 32);
   const int64_t at = (int64_t)split * own.rows_pad + own_row;
@@ -318,6 +377,7 @@ struct PrepSide {
   const float* bias;      // items: rows at -inf are not used
   char* img;
   float *inv, *h, *sgn;
+  int32_t* tgt;
   int vec;
 };
 
@@ -381,7 +441,10 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, 
   }
   if (q == 0) {
     if (NP == 2) s.inv[row] = inv;
-    if (s.sgn) s.sgn[row] = 1.f;
+    if (s.sgn) {
+      s.sgn[row] = 1.f;
+      s.tgt[row] = row < s.rows ? s.keep[row] : -1;
+    }
     s.h[row] = use && !s.keep ? bias * kLog2e - shift : -INFINITY;   // users: written once their normaliser is known
   }
 }
@@ -556,20 +619,29 @@ __global__ void __launch_bounds__(256) xent_table_kernel(TableOut a, Part part) 
 // ---- host --------------------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Splits of the stream axis: enough workgroups for two on every CU, at least two stages each; a multiple of 8 where there are as
-// many, so that the workgroups of one XCD (consecutive ids go round the eight of them) walk over the same part of the stream.
+// Splits of the stream axis: the launch runs in rounds of 512 workgroups (two on each of 256 CUs), each round as long as one split, which
+// costs its stages and about three more (operands in, results out and joined).  At 8,192 x 16,980 the backward pass has 133 own tiles:
+// 4 splits fill 1.04 rounds and took 210 us, 7 (two rounds, nearly full) TBD us.
 inline int splits_for(int64_t own_tiles, int64_t stream_tiles) {
-  int64_t s = up(512, own_tiles) / own_tiles;
-  s = std::min(s, std::max<int64_t>(1, stream_tiles / 2));
-  if (s > 8) s = s / 8 * 8;
-  return (int)std::min<int64_t>(s, 256);
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 256 && s <= stream_tiles; ++s) {
+    const int64_t per = (stream_tiles + s - 1) / s;
+    if (s > 1 && (stream_tiles + per - 1) / per != s) continue;    // the last split would be empty
+    const double cost = (double)((own_tiles * s + 511) / 512) * (double)(per + 3);
+    if (cost < least * 0.999) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 struct Layout {
   int np, dp;
   int64_t npad, cpad;
   int fs, bs;                       // splits of the two passes
-  int64_t u_img, u_inv, u_h, u_kq, u_sgn, v_img, v_inv, v_h, o, m, l, loss, valid, bytes;
+  int64_t u_img, u_inv, u_h, u_kq, u_sgn, u_tgt, v_img, v_inv, v_h, o, m, l, loss, valid, bytes;
 };
 
 Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
@@ -589,6 +661,7 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
   y.u_h = take(y.npad * 4);
   y.u_kq = take(y.npad * 4);
   y.u_sgn = take(y.npad * 4);
+  y.u_tgt = take(y.npad * 4);
   y.v_img = take(y.cpad * row);
   y.v_inv = take(y.cpad * 4);
   y.v_h = take(y.cpad * 4);
@@ -607,10 +680,11 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
   const bool grad = x->d_rows != nullptr;
   auto f = [ws](int64_t at) { return reinterpret_cast<float*>(ws + at); };
   int32_t* valid = reinterpret_cast<int32_t*>(ws + y.valid);
+  int32_t* tgt = reinterpret_cast<int32_t*>(ws + y.u_tgt);
   auto vec = [](const void* p, int64_t stride) { return ((uintptr_t)p % (4 * sizeof(E)) == 0 && stride % 4 == 0) ? 1 : 0; };
   const PrepSide pu{x->rows, x->rows_stride, x->n, y.npad, x->target, nullptr, ws + y.u_img, f(y.u_inv), f(y.u_h), f(y.u_sgn),
-                    vec(x->rows, x->rows_stride)};
-  const PrepSide pv{x->table, x->table_stride, x->c, y.cpad, nullptr, x->bias, ws + y.v_img, f(y.v_inv), f(y.v_h), nullptr,
+                    tgt, vec(x->rows, x->rows_stride)};
+  const PrepSide pv{x->table, x->table_stride, x->c, y.cpad, nullptr, x->bias, ws + y.v_img, f(y.v_inv), f(y.v_h), nullptr, nullptr,
                     vec(x->table, x->table_stride)};
   constexpr int kPrepRows = 256 / (DP / 8);
   const int64_t ub = up(y.npad, kPrepRows) / kPrepRows, vb = up(y.cpad, kPrepRows) / kPrepRows;
@@ -619,7 +693,7 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
     hipLaunchKernelGGL((xent_prep_kernel<E, NP, DP>), dim3((unsigned)(ub + vb + 1)), dim3(256), 0, st, pu, pv, ub, x->dim, valid,
                        (int)x->n);
   }
-  const Side u{ws + y.u_img, f(y.u_inv), f(y.u_h), f(y.u_kq), f(y.u_sgn), x->target, nullptr, x->n, y.npad};
+  const Side u{ws + y.u_img, f(y.u_inv), f(y.u_h), f(y.u_kq), f(y.u_sgn), tgt, nullptr, x->n, y.npad};
   const Side v{ws + y.v_img, f(y.v_inv), f(y.v_h), nullptr, nullptr, nullptr, x->bias, x->c, y.cpad};
   const Part part{f(y.o), f(y.m), f(y.l)};
   const float scale2 = x->scale * kLog2e;
