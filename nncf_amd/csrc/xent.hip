@@ -96,7 +96,7 @@ __device__ __forceinline__ int image_at(int i) {
 template <int NP, int DP>
 struct __attribute__((aligned(16))) Stage {
   char img[kTile * NP * DP * 2];
-  float h[kTile], inv[kTile], sgn[kTile];
+  float h[kTile], inv[kTile], sgn[kTile], kq[kTile];
   int32_t tgt[kTile];
 };
 typedef const __attribute__((address_space(1))) void* gptr_t;
@@ -128,6 +128,7 @@ __device__ __forceinline__ void fill(Stage<NP, DP>& to, const Filler<NP, DP>& f,
   }
   if (wave == 0) __builtin_amdgcn_global_load_lds((gptr_t)(str.h + row0 + lane), (lptr_t)to.h, 4, 0, 0);
   if (NP == 2 && wave == 1) __builtin_amdgcn_global_load_lds((gptr_t)(str.inv + row0 + lane), (lptr_t)to.inv, 4, 0, 0);
+  if (BWD && wave == 1) __builtin_amdgcn_global_load_lds((gptr_t)(str.kq + row0 + lane), (lptr_t)to.kq, 4, 0, 0);
   if (WT && wave == 2) __builtin_amdgcn_global_load_lds((gptr_t)(str.sgn + row0 + lane), (lptr_t)to.sgn, 4, 0, 0);
   if (BWD && wave == 3) __builtin_amdgcn_global_load_lds((gptr_t)(str.tgt + row0 + lane), (lptr_t)to.tgt, 4, 0, 0);
 }
@@ -156,10 +157,10 @@ __device__ __forceinline__ typename T::V read_cols(const char* lds, int plane, i
 
 // The streaming kernel.  BWD: own rows are items.  WT: row weights of either sign.  MEAN: the O sums are wanted.
 template <class T, int NP, int DP, bool BWD, bool WT, bool MEAN>
-__global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str, Part part, float scale2, int tiles, int tiles_per_split) {
+__global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str, Part part, float scale2, int stages, int stages_per_split) {
   typedef typename T::V V;
   constexpr int kRow = NP * DP * 2;             // bytes of an image row
-  constexpr int KS = DP / 16, DT = DP / 32;
+  constexpr int KS = DP / 16, DT = DP / 32, RT = NP == 2 || WT ? 1 : 2;   // sub-tiles of 32 stream rows worked on together
   __shared__ Stage<NP, DP> s_a, s_b;            // two objects, so that a read of one does not wait for the filling of the other
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int split = blockIdx.x;
@@ -183,63 +184,101 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
   float m = 0.f, l = 0.f;
   bool seen = false;
 
-  const int t0 = split * tiles_per_split, t1 = min(tiles, t0 + tiles_per_split);
   auto work = [&](const Stage<NP, DP>& st, int64_t row0) __attribute__((always_inline)) {
     const char* s_img = st.img;
-    const float *s_h = st.h, *s_inv = st.inv, *s_sgn = st.sgn;
+    const float *s_h = st.h, *s_inv = st.inv, *s_sgn = st.sgn, *s_kq = st.kq;
     const int32_t* s_tgt = st.tgt;
 #pragma unroll 1
-    for (int r = 0; r < kTile / 32; ++r) {
-      f32x16 s = 0.f;
+    for (int r0 = 0; r0 < kTile / 32; r0 += RT) {
+      f32x16 s[RT];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const V a = read_rows<T, NP, DP>(s_img, 32 * r + col, 0, 2 * k + half);
-        s = T::mfma(a, of[0][k], s);
-        if (NP == 2) {
-          const V b = read_rows<T, NP, DP>(s_img, 32 * r + col, 1, 2 * k + half);
-          s = T::mfma(a, of[NP - 1][k], s);
-          s = T::mfma(b, of[0][k], s);
-        }
-      }
-      float d[16], iv[16];
+      for (int r = 0; r < RT; ++r) s[r] = 0.f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int at = 32 * r + 8 * g + 4 * half;
-        const float4 h4 = *reinterpret_cast<const float4*>(s_h + at);
-        const float hv[4] = {h4.x, h4.y, h4.z, h4.w};
-        float4 i4 = make_float4(1.f, 1.f, 1.f, 1.f);
-        if (NP == 2) i4 = *reinterpret_cast<const float4*>(s_inv + at);
-        const float ivv[4] = {i4.x, i4.y, i4.z, i4.w};
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          iv[4 * g + e] = ivv[e];
-          d[4 * g + e] = fmaf(NP == 2 ? s[4 * g + e] * ivv[e] : s[4 * g + e], c, hv[e] - (m - add));
-        }
-      }
-      // targets: a wave-uniform branch, taken by one sub-tile in c / 32 per own row
-      uint32_t hit = 0;
-      if (!BWD) {
-        if (__any((uint32_t)(own_tgt - (int32_t)(row0 + 32 * r)) < 32u)) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if ((int32_t)(row0 + 32 * r) + 8 * (i >> 2) + 4 * half + (i & 3) == own_tgt) d[i] = -INFINITY;
-        }
-      } else {
-        const uint32_t in = (uint32_t)(s_tgt[32 * r + col] - (int32_t)own0);
-        if (__any(in < 32u)) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = 32 * r + 8 * (i >> 2) + 4 * half + (i & 3);
-            if (s_tgt[at] == own_id) {
-              hit |= 1u << i;
-              d[i] = __builtin_amdgcn_logf(fabsf(str.kq[row0 + at])) - m;
-            }
+        for (int r = 0; r < RT; ++r) {
+          const V a = read_rows<T, NP, DP>(s_img, 32 * (r0 + r) + col, 0, 2 * k + half);
+          s[r] = T::mfma(a, of[0][k], s[r]);
+          if (NP == 2) {
+            const V b = read_rows<T, NP, DP>(s_img, 32 * (r0 + r) + col, 1, 2 * k + half);
+            s[r] = T::mfma(a, of[NP - 1][k], s[r]);
+            s[r] = T::mfma(b, of[0][k], s[r]);
           }
         }
-      }
-      float top = d[0];
+      // operands three steps (NP == 1: eight) ahead of their products: left alone, the compiler read, waited and multiplied one by one, and a
+      // stage took 6,100 cycles for 1,024 of products
+      constexpr int kAhead = NP == 2 ? 6 : BWD ? 4 : 8, kReads = NP * KS * RT;
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, d[i]);
+      for (int i = kAhead; i < kReads; i += NP) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NP == 2 ? 3 : 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, NP == 2 ? 9 : kAhead, 0);
+      float d[RT][16], iv[NP == 2 ? RT : 1][16];
+      const float shift = m - add;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int at = 32 * (r0 + r) + 8 * g + 4 * half;
+          const float4 h4 = *reinterpret_cast<const float4*>(s_h + at);
+          const float hv[4] = {h4.x, h4.y, h4.z, h4.w};
+          float4 i4 = make_float4(1.f, 1.f, 1.f, 1.f);
+          if (NP == 2) i4 = *reinterpret_cast<const float4*>(s_inv + at);
+          const float ivv[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (NP == 2) iv[r][4 * g + e] = ivv[e];
+            d[r][4 * g + e] = fmaf(NP == 2 ? s[r][4 * g + e] * ivv[e] : s[r][4 * g + e], c, hv[e] - shift);
+          }
+        }
+      float top = d[0][0];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = r ? 0 : 1; i < 16; ++i) top = fmaxf(top, d[r][i]);
+      // targets: a wave-uniform branch, then selects: no lane loads or computes by itself
+      const int32_t first = (int32_t)(row0 + 32 * r0);
+      uint64_t hit_rows = 0;
+      if (!BWD) {
+        if (__any((uint32_t)(own_tgt - first) < 32u * RT)) {
+          top = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (first + 32 * r + 8 * (i >> 2) + 4 * half + (i & 3) == own_tgt) d[r][i] = -INFINITY;
+              top = fmaxf(top, d[r][i]);
+            }
+        }
+      } else {
+        // its own products, below; here a target's place holds nothing, and its size counts for the reference
+        hit_rows = __ballot((uint32_t)(s_tgt[32 * r0 + (RT == 2 ? lane : col)] - (int32_t)own0) < 32u);
+        if (hit_rows) {
+          top = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int at = 32 * (r0 + r) + 8 * g + 4 * half;
+              const int4 t4 = *reinterpret_cast<const int4*>(s_tgt + at);
+              const float4 k4 = *reinterpret_cast<const float4*>(s_kq + at);
+              const int32_t tv[4] = {t4.x, t4.y, t4.z, t4.w};
+              const float kv[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float& x = d[r][4 * g + e];
+                const bool is = tv[e] == own_id;
+                // 2^exponent is at or above the coefficient; one that is 0 asks for nothing
+                const float need = kv[e] == 0.f ? -INFINITY : (float)__builtin_amdgcn_frexp_expf(kv[e]) - m;
+                top = fmaxf(top, is ? need : x);
+                x = is ? -INFINITY : x;
+              }
+              __builtin_amdgcn_sched_barrier(0);   // the rare branch must not set the kernel's register count
+            }
+        }
+      }
       if (__any(top > kRaise || (!seen && top > -INFINITY))) {
         top = fmaxf(top, __shfl_xor(top, 32));   // both halves of a column keep one reference
         const bool move = top > kRaise || (!seen && top > -INFINITY);
@@ -249,76 +288,97 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
         m += by;
         l *= f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) d[i] -= by;
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d[r][i] -= by;
         if (MEAN) {
 #pragma unroll
           for (int t = 0; t < DT; ++t) o[t] *= f;
         }
       }
-      float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(d[i]);
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[r][i] = __builtin_amdgcn_exp2f(d[r][i]);
       if (WT) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 w4 = *reinterpret_cast<const float4*>(s_sgn + 32 * r + 8 * g + 4 * half);
-          p[4 * g] *= w4.x;
-          p[4 * g + 1] *= w4.y;
-          p[4 * g + 2] *= w4.z;
-          p[4 * g + 3] *= w4.w;
-        }
-      }
-      float plo[16];
-      if (BWD && NP == 1) {
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) plo[i] = 0.f;
-      }
-      const bool any_hit = BWD && __any(hit != 0);
-      if (any_hit) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (hit >> i & 1) {
-            p[i] = -ldexpf(str.kq[row0 + 32 * r + 8 * (i >> 2) + 4 * half + (i & 3)], (int)-m);
-            if (NP == 1) plo[i] = p[i] - (float)(typename T::E)p[i];
+          for (int g = 0; g < 4; ++g) {
+            const float4 w4 = *reinterpret_cast<const float4*>(s_sgn + 32 * (r0 + r) + 8 * g + 4 * half);
+            d[r][4 * g] *= w4.x;
+            d[r][4 * g + 1] *= w4.y;
+            d[r][4 * g + 2] *= w4.z;
+            d[r][4 * g + 3] *= w4.w;
           }
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        // 2^b = 1 / 2^-b, by its exponent
-        const float up = NP == 2 ? __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, iv[i])) : 1.f;
-        l = fmaf(p[i], up, l);
-      }
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          // 2^b = 1 / 2^-b, by its exponent
+          if (NP == 2) l = fmaf(d[r][i], __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, iv[r][i])), l);
+          else l += d[r][i];
+        }
       if (MEAN) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          V hi, lo;
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            hi[e] = (typename T::E)p[8 * q + e];
-            if (NP == 2) lo[e] = (typename T::E)(p[8 * q + e] - (float)hi[e]);
-          }
+          for (int q = 0; q < 2; ++q) {
+            V hi, lo;
 #pragma unroll
-          for (int t = 0; t < DT; ++t) {
-            const V a = read_cols<T, NP, DP>(s_img, 0, 32 * r + 16 * q, t, lane);
-            o[t] = T::mfma(a, hi, o[t]);
-            if (NP == 2) {
-              const V b = read_cols<T, NP, DP>(s_img, NP - 1, 32 * r + 16 * q, t, lane);
-              o[t] = T::mfma(a, lo, o[t]);
-              o[t] = T::mfma(b, hi, o[t]);
+            for (int e = 0; e < 8; ++e) {
+              hi[e] = (typename T::E)d[r][8 * q + e];
+              if (NP == 2) lo[e] = (typename T::E)(d[r][8 * q + e] - (float)hi[e]);
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+              const V a = read_cols<T, NP, DP>(s_img, 0, 32 * (r0 + r) + 16 * q, t, lane);
+              o[t] = T::mfma(a, hi, o[t]);
+              if (NP == 2) {
+                const V b = read_cols<T, NP, DP>(s_img, NP - 1, 32 * (r0 + r) + 16 * q, t, lane);
+                o[t] = T::mfma(a, lo, o[t]);
+                o[t] = T::mfma(b, hi, o[t]);
+              }
             }
           }
-          if (NP == 1 && any_hit) {   // one plane: what rounding took from a target's coefficient, the largest terms of its sum
+        if (BWD && hit_rows) {   // targets, 16 stream rows at a time: the largest terms of their sums, so two planes for every type
+#pragma unroll 1
+          for (int w = 0; w < 2 * RT; ++w) {
+            if (!(hit_rows >> (16 * w) & 0xffff)) continue;
+            V hi, lo;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) lo[e] = (typename T::E)plo[8 * q + e];
+            for (int g = 0; g < 2; ++g) {
+              const int at = 32 * r0 + 16 * w + 8 * g + 4 * half;
+              const int4 t4 = *reinterpret_cast<const int4*>(s_tgt + at);
+              const float4 k4 = *reinterpret_cast<const float4*>(s_kq + at);
+              float4 i4 = make_float4(1.f, 1.f, 1.f, 1.f);
+              if (NP == 2) i4 = *reinterpret_cast<const float4*>(s_inv + at);
+              const int32_t tv[4] = {t4.x, t4.y, t4.z, t4.w};
+              const float kv[4] = {k4.x, k4.y, k4.z, k4.w}, ivv[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
-            for (int t = 0; t < DT; ++t) o[t] = T::mfma(read_cols<T, NP, DP>(s_img, 0, 32 * r + 16 * q, t, lane), lo, o[t]);
+              for (int e = 0; e < 4; ++e) {
+                const float v = tv[e] == own_id ? -ldexpf(kv[e], (int)-m) : 0.f;
+                hi[4 * g + e] = (typename T::E)v;
+                lo[4 * g + e] = (typename T::E)(v - (float)hi[4 * g + e]);
+                l += NP == 2 ? v * __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, ivv[e])) : v;
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+              const V a = read_cols<T, NP, DP>(s_img, 0, 32 * r0 + 16 * w, t, lane);
+              o[t] = T::mfma(a, hi, o[t]);
+              o[t] = T::mfma(a, lo, o[t]);
+              if (NP == 2) o[t] = T::mfma(read_cols<T, NP, DP>(s_img, NP - 1, 32 * r0 + 16 * w, t, lane), hi, o[t]);
+            }
           }
         }
       }
     }
   };
-  const Filler<NP, DP> filler(wave, lane);
+  const int t0 = split * stages_per_split, t1 = min(stages, t0 + stages_per_split);
   if (t0 < t1) {
+    const Filler<NP, DP> filler(wave, lane);
     fill<NP, DP, BWD, WT>(s_a, filler, str, (int64_t)t0 * kTile, wave, lane);
     filled();
     for (int tile = t0; tile < t1; tile += 2) {
@@ -345,7 +405,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
         *reinterpret_cast<float4*>(part.o + at * DP + 32 * t + 8 * g + 4 * half) =
             make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
   }
-}
+  }
 
 // ---- images ------------------------------------------------------------------------------------------------------------------
 template <class E>
@@ -463,12 +523,15 @@ struct RowsOut {
   int d, mean, splits;
 };
 
-// One wave per row: joins its splits, adds the target, writes loss, lse, d_rows and what the row streams with in the backward pass.
-template <class E, int NP, int DP, bool MEAN>
+// W waves per row (1 or 4): joins its splits, adds the target, writes loss, lse, d_rows and what the row streams with in the backward
+// pass.  Reading a row's results of 128 splits in turn was a chain of trips to memory (15 us for any n): past 8 splits four waves share
+// them, eight reads in flight each.
+template <class E, int NP, int DP, bool MEAN, int W>
 __global__ void __launch_bounds__(256) xent_rows_kernel(RowsOut a, Part part) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.n) return;
+  __shared__ float s_o[W][DP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part_of = wave % W;
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
+  if (W == 1 && row >= a.n) return;
   const int32_t t = a.target[row];
   const bool has = t >= 0, bad = has && t >= a.c;
   const E* u = reinterpret_cast<const E*>(a.rows) + row * a.rows_stride;
@@ -487,14 +550,22 @@ __global__ void __launch_bounds__(256) xent_rows_kernel(RowsOut a, Part part) {
     }
     l = wave_sum(l);
     if (MEAN) {
-#pragma unroll 4
-      for (int k = 0; k < a.splits; ++k) {
+#pragma unroll 8
+      for (int k = part_of; k < a.splits; k += W) {
         const int64_t at = (int64_t)k * a.rows_pad + row;
         const float mk = part.m[at], f = mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - top) : 0.f;
         o0 = fmaf(part.o[at * DP + lane], f, o0);
         if (DP == 128) o1 = fmaf(part.o[at * DP + 64 + lane], f, o1);
       }
     }
+  }
+  if (W > 1) {
+    s_o[part_of][lane] = o0;
+    if (DP == 128) s_o[part_of][DP - 64 + lane] = o1;
+    __syncthreads();
+    if (part_of) return;
+    o0 = (s_o[0][lane] + s_o[1 % W][lane]) + (s_o[2 % W][lane] + s_o[3 % W][lane]);
+    if (DP == 128) o1 = (s_o[0][DP - 64 + lane] + s_o[1 % W][DP - 64 + lane]) + (s_o[2 % W][DP - 64 + lane] + s_o[3 % W][DP - 64 + lane]);
   }
   float u0 = 0.f, u1 = 0.f, v0 = 0.f, v1 = 0.f;
   const float beta = has && !bad && a.bias ? a.bias[t] : 0.f;
@@ -557,7 +628,7 @@ struct TableOut {
   float* d_bias;
   float scale;
   int64_t n, c, rows_pad;
-  int d, mean, splits, reduce;
+  int d, mean, reduce, splits;
 };
 
 // sum of the rows' losses, in row order per lane: one workgroup
@@ -619,17 +690,20 @@ __global__ void __launch_bounds__(256) xent_table_kernel(TableOut a, Part part) 
 // ---- host --------------------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Splits of the stream axis: the launch runs in rounds of 512 workgroups (two on each of 256 CUs), each round as long as one split, which
-// costs its stages and about three more (operands in, results out and joined).  At 8,192 x 16,980 the backward pass has 133 own tiles:
-// 4 splits fill 1.04 rounds and took 210 us, 7 (two rounds, nearly full) TBD us.
-inline int splits_for(int64_t own_tiles, int64_t stream_tiles) {
+// Splits of the stream axis.  A launch runs in rounds of 512 workgroups (two on each of 256 CUs); a split costs its stages and about three
+// more (operands in, results out and joined).  In the backward pass a popular item's workgroup meets a target in every stage and takes
+// twice as long in it: it may become the launch's long pole.  Measured, backward: 1,000 x 50,021 f16 (391 own tiles, 16 stages) 97 us
+// with 1 split, 56 with 2, 76 with 8; 512 x 17,000 fp32 (133, 8) 56 / 37 / 31 / 33 / 39 us with 1 / 2 / 3 / 4 / 8; forward: 512 rows (4 own
+// tiles, 266 stages) 102 / 57 / 36 / 26 / 31 us with 8 / 16 / 32 / 64 / 256.
+inline int splits_for(int64_t own_tiles, int64_t stages, bool backward) {
   int best = 1;
-  double least = 1e30;
-  for (int s = 1; s <= 256 && s <= stream_tiles; ++s) {
-    const int64_t per = (stream_tiles + s - 1) / s;
-    if (s > 1 && (stream_tiles + per - 1) / per != s) continue;    // the last split would be empty
-    const double cost = (double)((own_tiles * s + 511) / 512) * (double)(per + 3);
-    if (cost < least * 0.999) {
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 256 && s <= stages; ++s) {
+    const int64_t per = (stages + s - 1) / s;
+    if ((stages + per - 1) / per != s) continue;    // the last split would be empty
+    const int64_t rounds = (own_tiles * s + 511) / 512;
+    const int64_t cost = std::max(rounds * (per + 3), backward ? 2 * per + 3 : 0);
+    if (cost < least) {
       least = cost;
       best = s;
     }
@@ -650,8 +724,8 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
   y.dp = d <= 64 ? 64 : 128;
   y.npad = up(n, kOwn);
   y.cpad = up(c, kOwn);
-  y.fs = splits_for(y.npad / kOwn, up(c, kTile) / kTile);
-  y.bs = splits_for(y.cpad / kOwn, up(n, kTile) / kTile);
+  y.fs = splits_for(y.npad / kOwn, up(c, kTile) / kTile, false);
+  y.bs = splits_for(y.cpad / kOwn, up(n, kTile) / kTile, true);
   int64_t at = 0;
   auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };
   const int64_t row = (int64_t)y.np * y.dp * 2;
@@ -698,13 +772,13 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
   const Part part{f(y.o), f(y.m), f(y.l)};
   const float scale2 = x->scale * kLog2e;
   {
-    const int tiles = (int)(up(x->c, kTile) / kTile), per = (tiles + y.fs - 1) / y.fs;
+    const int stages = (int)(up(x->c, kTile) / kTile), per = (stages + y.fs - 1) / y.fs;
     const dim3 grid((unsigned)y.fs, (unsigned)(y.npad / kOwn));
     ProfScope ps("xent_stream_kernel", st);
     if (grad)
-      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, true>), grid, dim3(256), 0, st, u, v, part, scale2, tiles, per);
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, true>), grid, dim3(256), 0, st, u, v, part, scale2, stages, per);
     else
-      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, false>), grid, dim3(256), 0, st, u, v, part, scale2, tiles, per);
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, false>), grid, dim3(256), 0, st, u, v, part, scale2, stages, per);
   }
   const bool scalar = x->reduction != NNCF_NONE;
   const int mean = x->reduction == NNCF_MEAN;
@@ -713,24 +787,25 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
                    grad ? f(y.u_h) : nullptr, f(y.u_kq), f(y.u_sgn), f(y.u_inv), x->d_rows, x->scale, x->n, x->c, y.npad, x->dim, mean, y.fs};
   {
     ProfScope ps("xent_rows_kernel", st);
-    const dim3 grid((unsigned)((x->n + 3) / 4));
-    if (grad)
-      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, true>), grid, dim3(256), 0, st, ro, part);
+    if (!grad)
+      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, false, 1>), dim3((unsigned)((x->n + 3) / 4)), dim3(256), 0, st, ro, part);
+    else if (y.fs <= 8)
+      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, true, 1>), dim3((unsigned)((x->n + 3) / 4)), dim3(256), 0, st, ro, part);
     else
-      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, false>), grid, dim3(256), 0, st, ro, part);
+      hipLaunchKernelGGL((xent_rows_kernel<E, NP, DP, true, 4>), dim3((unsigned)x->n), dim3(256), 0, st, ro, part);
   }
-  TableOut to{x->bias, valid, loss_rows, x->loss, x->d_table, x->d_bias, x->scale, x->n, x->c, y.cpad, x->dim, mean, y.bs, scalar};
+  TableOut to{x->bias, valid, loss_rows, x->loss, x->d_table, x->d_bias, x->scale, x->n, x->c, y.cpad, x->dim, mean, scalar, y.bs};
   if (!grad) {
     if (scalar) hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, st, to);
   } else {
-    const int tiles = (int)(up(x->n, kTile) / kTile), per = (tiles + y.bs - 1) / y.bs;
+    const int stages = (int)(up(x->n, kTile) / kTile), per = (stages + y.bs - 1) / y.bs;
     const dim3 grid((unsigned)y.bs, (unsigned)(y.cpad / kOwn));
     {
       ProfScope ps("xent_stream_kernel", st);
       if (x->weight)
-        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, true, true>), grid, dim3(256), 0, st, v, u, part, scale2, tiles, per);
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, true, true>), grid, dim3(256), 0, st, v, u, part, scale2, stages, per);
       else
-        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, false, true>), grid, dim3(256), 0, st, v, u, part, scale2, tiles, per);
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, false, true>), grid, dim3(256), 0, st, v, u, part, scale2, stages, per);
     }
     ProfScope ps("xent_table_kernel", st);
     constexpr int kRows = 256 / (DP / 4);
