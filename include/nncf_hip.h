@@ -626,6 +626,13 @@ int nncf_dequantize_rows(const int8_t* d_q, const float* d_scale, int64_t n, int
 int nncf_int8_scores(const int8_t* d_qx, const float* d_sx, int64_t m, const int8_t* d_qt, const float* d_st, int64_t c, int32_t k,
                      const float* d_row_bias, const float* d_col_bias, void* d_out, int64_t out_stride, int32_t dtype, void* stream);
 
+/* The same for m float rows that are coded on the way, in ONE launch: for the few rows with nncf_int8_scores_fused(m, k) != 0 (m <= 32 and
+ * m * nncf_int8_pitch(k) <= 4096; others are refused: nncf_quantize_rows first). */
+int32_t nncf_int8_scores_fused(int64_t m, int32_t k);
+int nncf_int8_scores_rows(const void* d_x, int64_t x_stride, int32_t x_dtype, int64_t m, const int8_t* d_qt, const float* d_st, int64_t c,
+                          int32_t k, const float* d_row_bias, const float* d_col_bias, void* d_out, int64_t out_stride, int32_t dtype,
+                          void* stream);
+
 /* Row movers and routing of the sharded path (no reference counterpart).
  * nncf_shard_route: for a batch's item ids d_cid[n], with item rows owned by rank id / item_shard:
  *   d_req[n_ranks][cap] = the unique ids to request from each owner (ascending, -1 padded) and

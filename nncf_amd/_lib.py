@@ -195,6 +195,8 @@ def _declare(lib):
         "nncf_quantize_rows": [vp, i64, i32, i64, i32, i32, vp, vp, vp],
         "nncf_dequantize_rows": [vp, vp, i64, i32, vp, i32, vp],
         "nncf_int8_scores": [vp, vp, i64, vp, vp, i64, i32, vp, vp, vp, i64, i32, vp],
+        "nncf_int8_scores_fused": [i64, i32],
+        "nncf_int8_scores_rows": [vp, i64, i32, i64, vp, vp, i64, i32, vp, vp, vp, i64, i32, vp],
         "nncf_plan_ids": [vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp],
     })
     for name, args in sig.items():

@@ -54,7 +54,7 @@ def _vector(t, name, n, dtype, device):
 
 
 def _call(device, fn, *args):
-    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    stream = torch.cuda.current_stream(device).cuda_stream
     if torch.cuda.current_device() == device.index:
         _lib.check(fn(*args, stream))
     else:
@@ -112,7 +112,7 @@ def softmax_xent(rows, table, target, bias=None, weight=None, scale=1.0, reducti
         if bias is not None:
             d_bias = torch.empty(c, dtype=torch.float32, device=device)
             x.d_bias = d_bias.data_ptr()
-    _call(device, L.nncf_softmax_xent, ctypes.byref(x), ctypes.c_void_p(ws.data_ptr()), ws_bytes)
+    _call(device, L.nncf_softmax_xent, ctypes.byref(x), ws.data_ptr(), ws_bytes)
     return XentResult(loss, lse, d_rows, d_table, d_bias)
 
 
@@ -133,8 +133,8 @@ class Int8Rows(object):
         if dtype not in _DTYPES:
             raise TypeError("dtype %s" % (dtype,))
         out = torch.empty((len(self), self.k), dtype=dtype, device=self.codes.device)
-        _call(out.device, _lib.lib().nncf_dequantize_rows, ctypes.c_void_p(self.codes.data_ptr()), ctypes.c_void_p(self.scale.data_ptr()),
-              len(self), self.k, ctypes.c_void_p(out.data_ptr()), _DTYPES[dtype])
+        _call(out.device, _lib.lib().nncf_dequantize_rows, self.codes.data_ptr(), self.scale.data_ptr(),
+              len(self), self.k, out.data_ptr(), _DTYPES[dtype])
         return out
 
 
@@ -150,8 +150,8 @@ def quantize_rows(x, normalize=False):
         raise ValueError("rows of %d columns (1 .. 131072)" % k)
     codes = torch.empty((n, pitch), dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
-    _call(x.device, L.nncf_quantize_rows, ctypes.c_void_p(x.data_ptr()), _pitch(x), _DTYPES[x.dtype], n, k, int(bool(normalize)),
-          ctypes.c_void_p(codes.data_ptr()), ctypes.c_void_p(scale.data_ptr()))
+    _call(x.device, L.nncf_quantize_rows, x.data_ptr(), _pitch(x), _DTYPES[x.dtype], n, k, int(bool(normalize)),
+          codes.data_ptr(), scale.data_ptr())
     return Int8Rows(codes, scale, k)
 
 
@@ -164,14 +164,19 @@ def int8_scores(rows, table, row_bias=None, col_bias=None, out=None, dtype=torch
     stride (or a new tensor of `dtype`)."""
     if not isinstance(table, Int8Rows):
         raise TypeError("table must be Int8Rows (quantize_rows)")
-    if not isinstance(rows, Int8Rows):
-        rows = quantize_rows(rows)
-    m, c, k = len(rows), len(table), table.k
+    L = _lib.lib()
+    c, k = len(table), table.k
     device = table.codes.device
-    if rows.k != k:
-        raise ValueError("rows are %d wide, the table %d" % (rows.k, k))
-    if rows.codes.device != device:
-        raise TypeError("rows are on %s, the table on %s" % (rows.codes.device, device))
+    coded = isinstance(rows, Int8Rows)
+    if not coded:
+        _matrix(rows, "rows", _DTYPES)
+        if rows.shape[1] == k and not L.nncf_int8_scores_fused(rows.shape[0], k):
+            rows, coded = quantize_rows(rows), True
+    m, width, where = (len(rows), rows.k, rows.codes.device) if coded else (rows.shape[0], rows.shape[1], rows.device)
+    if width != k:
+        raise ValueError("rows are %d wide, the table %d" % (width, k))
+    if where != device:
+        raise TypeError("rows are on %s, the table on %s" % (where, device))
     if out is None:
         if dtype not in _DTYPES:
             raise TypeError("dtype %s" % (dtype,))
@@ -180,9 +185,10 @@ def int8_scores(rows, table, row_bias=None, col_bias=None, out=None, dtype=torch
         _matrix(out, "out", _DTYPES)
         if out.device != device or tuple(out.shape) != (m, c):
             raise ValueError("out must be [%d, %d] on %s" % (m, c, device))
-    _call(device, _lib.lib().nncf_int8_scores, ctypes.c_void_p(rows.codes.data_ptr()), ctypes.c_void_p(rows.scale.data_ptr()), m,
-          ctypes.c_void_p(table.codes.data_ptr()), ctypes.c_void_p(table.scale.data_ptr()), c, k,
-          ctypes.c_void_p(_vector(row_bias, "row_bias", m, torch.float32, device)),
-          ctypes.c_void_p(_vector(col_bias, "col_bias", c, torch.float32, device)),
-          ctypes.c_void_p(out.data_ptr()), _pitch(out), _DTYPES[out.dtype])
+    rest = (table.codes.data_ptr(), table.scale.data_ptr(), c, k, _vector(row_bias, "row_bias", m, torch.float32, device),
+            _vector(col_bias, "col_bias", c, torch.float32, device), out.data_ptr(), _pitch(out), _DTYPES[out.dtype])
+    if coded:
+        _call(device, L.nncf_int8_scores, rows.codes.data_ptr(), rows.scale.data_ptr(), m, *rest)
+    else:
+        _call(device, L.nncf_int8_scores_rows, rows.data_ptr(), _pitch(rows), _DTYPES[rows.dtype], m, *rest)
     return out

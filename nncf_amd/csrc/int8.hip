@@ -133,89 +133,216 @@ struct Scores {
   int64_t m, c, out_stride, pitch;
 };
 
-// ---- many rows: 128 x 128 outputs per workgroup, 64 x 64 per wave, k in steps of KB bytes through LDS ------------------------------
-constexpr int kMT = 128;
+// ---- many rows ---------------------------------------------------------------------------------------------------------------
+// (64 WM) x (64 WC) outputs per workgroup, (32 WM) x (32 WC) per wave, 64 codes a stage, two stages in turn, filled from global memory
+// without a register (1 KB per wave and instruction: 16 rows of 64 bytes).  Chunks of 16 bytes lie at chunk ^ (row / 4 % 4): the 32 rows
+// of an operand read meet every bank alike.
+typedef const __attribute__((address_space(1))) void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
 
-template <int KB>
-__device__ __forceinline__ int tile_at(int row, int chunk) {   // 16-byte chunks; see the bank note at the reads
-  if (KB == 128) return row * 128 + ((chunk ^ (row >> 1 & 7)) << 4);
-  return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4);
+__device__ __forceinline__ int at64(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4); }
+
+template <int WM, int WC>
+struct __attribute__((aligned(16))) CodeStage {
+  char x[64 * WM * 64], t[64 * WC * 64];
+};
+
+template <class E, int WM, int WC, bool ONE>
+__global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t c_tiles, int64_t tiles, int vec) {
+  constexpr int MT = 64 * WM, CT = 64 * WC, NX = WM, NT = WC;   // NX + NT fills of 16 rows per wave and stage
+  __shared__ CodeStage<WM, WC> s_a, s_b;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  // Workgroups of an XCD (ids of one residue mod 8) take neighbouring tiles of the same rows, so that its L2 sees whole lines of the output
+  const int64_t share = (tiles + 7) / 8, tile = (int64_t)(blockIdx.x % 8) * share + blockIdx.x / 8;
+  if (tile >= tiles) return;
+  const int64_t m0 = tile / c_tiles * MT, c0 = tile % c_tiles * CT;
+  const int8_t *gx = a.qx + m0 * a.pitch, *gt = a.qt + c0 * a.pitch;
+  const int mrows = (int)min((int64_t)MT, a.m - m0), crows = (int)min((int64_t)CT, a.c - c0);
+  // rows behind the last are read as the last
+  uint32_t ox[NX], ot[NT];
+  const int frow = lane >> 2, fchunk = ((lane & 3) ^ (lane >> 4 & 3)) << 4;
+#pragma unroll
+  for (int i = 0; i < NX; ++i) ox[i] = (uint32_t)min((wave * NX + i) * 16 + frow, mrows - 1) * (uint32_t)a.pitch + fchunk;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) ot[i] = (uint32_t)min((wave * NT + i) * 16 + frow, crows - 1) * (uint32_t)a.pitch + fchunk;
+  auto fill = [&](CodeStage<WM, WC>& st, int64_t k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) __builtin_amdgcn_global_load_lds((gptr_t)(gx + k0 + ox[i]), (lptr_t)(st.x + (wave * NX + i) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) __builtin_amdgcn_global_load_lds((gptr_t)(gt + k0 + ot[i]), (lptr_t)(st.t + (wave * NT + i) * 1024), 16, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);   // asked for before the products of the stage, not among them
+  };
+  auto filled = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  const int wm = (wave >> 1) * 32 * WM, wc = (wave & 1) * 32 * WC;
+  i32x16 acc[WM][WC];
+#pragma unroll
+  for (int i = 0; i < WM; ++i)
+#pragma unroll
+    for (int j = 0; j < WC; ++j) acc[i][j] = 0;
+  auto work = [&](const CodeStage<WM, WC>& st) __attribute__((always_inline)) {
+    i32x4 x[2][WM], t[2][WC];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < WM; ++i) x[k][i] = *reinterpret_cast<const i32x4*>(st.x + at64(wm + 32 * i + col, 2 * k + half));
+#pragma unroll
+      for (int j = 0; j < WC; ++j) t[k][j] = *reinterpret_cast<const i32x4*>(st.t + at64(wc + 32 * j + col, 2 * k + half));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < WC; ++j)
+#pragma unroll
+        for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[k][i], t[k][j], acc[i][j], 0, 0, 0);
+  };
+  fill(s_a, 0);
+  filled();
+  if constexpr (ONE) {
+    work(s_a);
+    __syncthreads();
+  } else {
+    for (int64_t k0 = 0; k0 < a.pitch; k0 += 128) {   // a pitch above 64 is a multiple of 128
+      fill(s_b, k0 + 64);
+      work(s_a);
+      filled();
+      if (k0 + 128 < a.pitch) fill(s_a, k0 + 128);
+      work(s_b);
+      filled();
+    }
+  }
+  // A wave's 32 x 32 blocks: to rows of 4 adjacent values per lane by way of LDS (8 x 128 bytes per store instruction), where the
+  // output allows it.
+  float* turn = reinterpret_cast<float*>(s_a.x) + wave * (32 * 40);
+  static_assert(sizeof(s_a) >= 4 * 32 * 40 * 4 || WM * WC == 1, "room to turn a block per wave");
+#pragma unroll
+  for (int i = 0; i < WM; ++i) {
+    float sx[16], rb[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t row = min(m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3), a.m - 1);
+      sx[r] = a.sx[row];
+      rb[r] = a.rb ? a.rb[row] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < WC; ++j) {
+      __builtin_amdgcn_sched_barrier(0);   // block by block: the next one's scales would take the registers of its sums
+      const int64_t item = c0 + wc + 32 * j + col, safe = min(item, a.c - 1);
+      const float st = a.st[safe], cb = a.cb ? a.cb[safe] : 0.f;
+      float v[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = ((float)acc[i][j][r] * sx[r]) * st + (rb[r] + cb);
+      if (vec && WM * WC > 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) turn[(8 * (r >> 2) + 4 * half + (r & 3)) * 40 + col] = v[r];
+        __builtin_amdgcn_wave_barrier();
+        const int64_t c4 = c0 + wc + 32 * j + 4 * (lane & 7);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int in = 8 * q + (lane >> 3);
+          const int64_t row = m0 + wm + 32 * i + in;
+          const float4 f = *reinterpret_cast<const float4*>(turn + in * 40 + 4 * (lane & 7));
+          if (row < a.m && c4 < a.c) {   // c is a multiple of 4 here
+            typedef E E4 __attribute__((ext_vector_type(4)));
+            E4 o;
+            o[0] = (E)f.x;
+            o[1] = (E)f.y;
+            o[2] = (E)f.z;
+            o[3] = (E)f.w;
+            *reinterpret_cast<E4*>(reinterpret_cast<E*>(a.out) + row * a.out_stride + c4) = o;
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      } else if (item < a.c) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int64_t row = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (row < a.m) reinterpret_cast<E*>(a.out)[row * a.out_stride + item] = (E)v[r];
+        }
+      }
+    }
+  }
 }
 
-template <class E, int KB>
-__global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t m_tiles) {
-  __shared__ __attribute__((aligned(16))) char s_x[kMT * KB], s_t[kMT * KB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int64_t m0 = (int64_t)(blockIdx.x % m_tiles) * kMT, c0 = (int64_t)(blockIdx.x / m_tiles) * kMT;
-  const int wm = (wave >> 1) * 64, wc = (wave & 1) * 64;
-  i32x16 acc[2][2];
+// ---- up to 32 rows: the table is read once, straight into the operands -------------------------------------------------------------
+// A wave takes 32 items at a time, four times (16 reads of 1 KB in flight for rows of 128 codes), against all rows, which it holds.
+// FUSED: the rows come as floating point values, and every workgroup codes them for itself (m k <= kFused values) instead of waiting
+// for a launch that does it once.
+constexpr int kFused = 4096;
+
+struct FloatRows {
+  const void* x;
+  int64_t stride, k;
+  int vec;
+};
+
+template <class E, class X, bool FUSED>
+__global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRows f) {
+  __shared__ __attribute__((aligned(16))) int8_t s_q[FUSED ? kFused : 16];
+  __shared__ float s_sx[32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+  const int8_t* qx = a.qx;
+  const float* sx = a.sx;
+  if constexpr (FUSED) {
+    for (int r = wave; r < a.m; r += 4) {
+      const X* src = reinterpret_cast<const X*>(f.x) + r * f.stride;
+      float v[8], top = 0.f, sum2 = 0.f;
+      bool finite = true;
+      for (int64_t c0 = 8 * lane; c0 < a.pitch; c0 += 512) {
+        load8(src, c0, f.k, f.vec != 0, v);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+        for (int e = 0; e < 8; ++e) {
+          finite = finite && fabsf(v[e]) < INFINITY;
+          top = fmaxf(top, fabsf(v[e]));
+        }
+      }
+      int ok = finite;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = 0;
-  for (int64_t k0 = 0; k0 < a.pitch; k0 += KB) {
-    __syncthreads();
-    for (int i = tid; i < kMT * KB / 16; i += 256) {
-      const int row = i / (KB / 16), chunk = i % (KB / 16);
-      const int64_t rx = std::min(m0 + row, a.m - 1), rt = std::min(c0 + row, a.c - 1);
-      *reinterpret_cast<int4*>(s_x + tile_at<KB>(row, chunk)) = *reinterpret_cast<const int4*>(a.qx + rx * a.pitch + k0 + chunk * 16);
-      *reinterpret_cast<int4*>(s_t + tile_at<KB>(row, chunk)) = *reinterpret_cast<const int4*>(a.qt + rt * a.pitch + k0 + chunk * 16);
+      for (int o = 32; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, o));
+        ok &= __shfl_xor(ok, o);
+      }
+      const Coder c = coder_for(top, ok != 0, sum2, 0);
+      for (int64_t c0 = 8 * lane; c0 < a.pitch; c0 += 512) {
+        if (a.pitch > 512) load8(src, c0, f.k, f.vec != 0, v);
+        *reinterpret_cast<uint64_t*>(s_q + r * a.pitch + c0) = codes8(v, c);
+      }
+      if (lane == 0) s_sx[r] = c.scale;
     }
     __syncthreads();
+    qx = s_q;
+    sx = s_sx;
+  }
+  const int8_t* x = qx + min((int64_t)col, a.m - 1) * a.pitch + half * 16;
+  const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * 128;
+  if (first >= a.c) return;
+  const int8_t* t[4];
+  i32x16 acc[4];
 #pragma unroll
-    for (int k = 0; k < KB / 32; ++k) {
-      i32x4 x[2], t[2];
+  for (int j = 0; j < 4; ++j) {
+    t[j] = a.qt + min(first + 32 * j + col, a.c - 1) * a.pitch + half * 16;
+    acc[j] = 0;
+  }
+  for (int64_t k0 = 0; k0 < a.pitch; k0 += 64) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        x[i] = *reinterpret_cast<const i32x4*>(s_x + tile_at<KB>(wm + 32 * i + col, 2 * k + half));
-        t[i] = *reinterpret_cast<const i32x4*>(s_t + tile_at<KB>(wc + 32 * i + col, 2 * k + half));
-      }
+    for (int k = 0; k < 2; ++k) {
+      const i32x4 xk = *reinterpret_cast<const i32x4*>(x + k0 + 32 * k);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], t[j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xk, *reinterpret_cast<const i32x4*>(t[j] + k0 + 32 * k), acc[j], 0, 0, 0);
     }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t item = c0 + wc + 32 * j + col;
+  for (int j = 0; j < 4; ++j) {
+    const int64_t item = first + 32 * j + col;
     if (item >= a.c) continue;
     const float st = a.st[item], cb = a.cb ? a.cb[item] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (row < a.m) {
-          const float v = ((float)acc[i][j][r] * a.sx[row]) * st + (a.rb ? a.rb[row] + cb : cb);
-          reinterpret_cast<E*>(a.out)[row * a.out_stride + item] = (E)v;
-        }
-      }
-  }
-}
-
-// ---- up to 32 rows: the table is read once, 32 items per wave straight into the operands ------------------------------------------
-template <class E>
-__global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int64_t c0 = ((int64_t)blockIdx.x * 4 + wave) * 32;
-  if (c0 >= a.c) return;
-  const int8_t* t = a.qt + std::min(c0 + col, a.c - 1) * a.pitch + half * 16;
-  const int8_t* x = a.qx + std::min<int64_t>(col, a.m - 1) * a.pitch + half * 16;
-  i32x16 acc = 0;
-  for (int64_t k0 = 0; k0 < a.pitch; k0 += 64) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const i32x4*>(t + k0 + 32 * k),
-                                                  *reinterpret_cast<const i32x4*>(x + k0 + 32 * k), acc, 0, 0, 0);
-  }
-  if (col >= a.m) return;
-  const float sx = a.sx[col], rb = a.rb ? a.rb[col] : 0.f;
-  E* out = reinterpret_cast<E*>(a.out) + (int64_t)col * a.out_stride;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int64_t item = c0 + 8 * (r >> 2) + 4 * half + (r & 3);
-    if (item < a.c) out[item] = (E)(((float)acc[r] * sx) * a.st[item] + (a.cb ? rb + a.cb[item] : rb));
+    for (int r = 0; r < 16; ++r) {
+      const int row = 8 * (r >> 2) + 4 * half + (r & 3);
+      if (row < a.m) reinterpret_cast<E*>(a.out)[row * a.out_stride + item] = (E)(((float)acc[j][r] * sx[row]) * st + (a.rb ? a.rb[row] + cb : cb));
+    }
   }
 }
 
@@ -235,21 +362,42 @@ int run_quantize(const void* x, int64_t stride, int64_t n, int64_t k, int normal
   return NNCF_OK;
 }
 
-template <class E>
-int run_scores(const Scores& a, hipStream_t st) {
+template <class E, class X, bool FUSED>
+int run_few(const Scores& a, const FloatRows& f, hipStream_t st) {
   ProfScope ps("int8_scores_kernel", st);
-  if (a.m <= 32) {
-    hipLaunchKernelGGL((int8_scores_few_kernel<E>), dim3((unsigned)((a.c + 127) / 128)), dim3(256), 0, st, a);
-  } else {
-    const int64_t mt = (a.m + kMT - 1) / kMT, ct = (a.c + kMT - 1) / kMT;
-    NNCF_REQUIRE(mt * ct < (1LL << 31), "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
-    if (a.pitch == 64)
-      hipLaunchKernelGGL((int8_scores_kernel<E, 64>), dim3((unsigned)(mt * ct)), dim3(256), 0, st, a, mt);
-    else
-      hipLaunchKernelGGL((int8_scores_kernel<E, 128>), dim3((unsigned)(mt * ct)), dim3(256), 0, st, a, mt);
-  }
+  hipLaunchKernelGGL((int8_scores_few_kernel<E, X, FUSED>), dim3((unsigned)((a.c + 511) / 512)), dim3(256), 0, st, a, f);
   NNCF_HIP_CHECK(hipGetLastError());
   return NNCF_OK;
+}
+
+template <class E, int WM, int WC>
+int run_many(const Scores& a, hipStream_t st) {
+  const int64_t mt = (a.m + 64 * WM - 1) / (64 * WM), ct = (a.c + 64 * WC - 1) / (64 * WC);
+  NNCF_REQUIRE(mt * ct < (1LL << 30), "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
+  const int vec = a.c % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(E)) == 0;
+  ProfScope ps("int8_scores_kernel", st);
+  const dim3 grid((unsigned)((mt * ct + 7) / 8 * 8));
+  if (a.pitch == 64)
+    hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC, true>), grid, dim3(256), 0, st, a, ct, mt * ct, vec);
+  else
+    hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC, false>), grid, dim3(256), 0, st, a, ct, mt * ct, vec);
+  NNCF_HIP_CHECK(hipGetLastError());
+  return NNCF_OK;
+}
+
+template <class E>
+int run_scores(const Scores& a, hipStream_t st) {
+  if (a.m <= 32) return run_few<E, float, false>(a, FloatRows{}, st);
+  // large tiles once they are enough for every CU
+  const int64_t large = (a.m + 127) / 128 * ((a.c + 255) / 256);
+  return large >= 256 ? run_many<E, 2, 4>(a, st) : run_many<E, 1, 1>(a, st);
+}
+
+template <class E>
+int run_fused(const Scores& a, const FloatRows& f, int32_t x_dtype, hipStream_t st) {
+  if (x_dtype == NNCF_F32) return run_few<E, float, true>(a, f, st);
+  if (x_dtype == NNCF_F16) return run_few<E, _Float16, true>(a, f, st);
+  return run_few<E, __bf16, true>(a, f, st);
 }
 
 bool known(int32_t dtype) { return dtype == NNCF_F32 || dtype == NNCF_F16 || dtype == NNCF_BF16; }
@@ -317,4 +465,29 @@ extern "C" int nncf_int8_scores(const int8_t* d_qx, const float* d_sx, int64_t m
   if (dtype == NNCF_F32) return run_scores<float>(a, st);
   if (dtype == NNCF_F16) return run_scores<_Float16>(a, st);
   return run_scores<__bf16>(a, st);
+}
+
+extern "C" int32_t nncf_int8_scores_fused(int64_t m, int32_t k) {
+  return m > 0 && m <= 32 && k > 0 && k <= nncf::kMaxDepth && m * nncf::pitch_of(k) <= nncf::kFused;
+}
+
+extern "C" int nncf_int8_scores_rows(const void* d_x, int64_t x_stride, int32_t x_dtype, int64_t m, const int8_t* d_qt, const float* d_st,
+                                     int64_t c, int32_t k, const float* d_row_bias, const float* d_col_bias, void* d_out, int64_t out_stride,
+                                     int32_t dtype, void* stream) {
+  using namespace nncf;
+  NNCF_REQUIRE(nncf_int8_scores_fused(m, k), "%lld rows of %d columns are coded by nncf_quantize_rows first", (long long)m, k);
+  NNCF_REQUIRE(c >= 0 && c <= (1LL << 31), "c = %lld out of range", (long long)c);
+  NNCF_REQUIRE(known(dtype) && known(x_dtype), "dtype = %d or %d unknown", dtype, x_dtype);
+  if (c == 0) return NNCF_OK;
+  NNCF_REQUIRE(d_x && d_qt && d_st && d_out, "NULL argument");
+  NNCF_REQUIRE(x_stride >= k, "row stride %lld is below k = %d", (long long)x_stride, k);
+  NNCF_REQUIRE(((uintptr_t)d_qt & 15) == 0, "codes must be 16-byte aligned");
+  NNCF_REQUIRE((uintptr_t)d_x % size_of(x_dtype) == 0 && (uintptr_t)d_out % size_of(dtype) == 0, "a tensor is not aligned to its elements");
+  NNCF_REQUIRE(out_stride >= c, "output stride %lld is below c = %lld", (long long)out_stride, (long long)c);
+  const Scores a{nullptr, d_qt, nullptr, d_st, d_row_bias, d_col_bias, d_out, m, c, out_stride, pitch_of(k)};
+  const FloatRows f{d_x, x_stride, k, (uintptr_t)d_x % (4 * size_of(x_dtype)) == 0 && x_stride % 4 == 0};
+  hipStream_t st = as_stream(stream);
+  if (dtype == NNCF_F32) return run_fused<float>(a, f, x_dtype, st);
+  if (dtype == NNCF_F16) return run_fused<_Float16>(a, f, x_dtype, st);
+  return run_fused<__bf16>(a, f, x_dtype, st);
 }

@@ -64,6 +64,16 @@ def test_scores_refuse(i, v, word):
         _lib.check(_lib.lib().nncf_int8_scores(*args))
 
 
+@pytest.mark.parametrize("i,v,word", [(0, None, "NULL"), (1, 9, "stride"), (2, 3, "dtype"), (3, 33, "first"), (3, 0, "first"), (4, None, "NULL"),
+                                      (5, None, "NULL"), (6, -1, "out of range"), (7, 0, "first"), (7, 4097, "first"), (10, None, "NULL"),
+                                      (11, 99, "stride"), (12, 7, "dtype"), (0, P + 2, "aligned"), (4, P + 8, "aligned"), (10, P + 1, "aligned")])
+def test_scores_of_float_rows_refuse(i, v, word):
+    args = [P, 10, 0, 4, P, P, 100, 10, None, None, P, 100, 0, None]
+    args[i] = v
+    with pytest.raises(ValueError, match=word):
+        _lib.check(_lib.lib().nncf_int8_scores_rows(*args))
+
+
 def test_dequantize_refuses():
     L = _lib.lib()
     for args in ([None, P, 4, 10, P, 0, None], [P, P, 4, 0, P, 0, None], [P, P, 4, 10, P, 3, None], [P, P, 4, 10, P + 4, 0, None], [P, P, -1, 10, P, 0, None]):
