@@ -54,7 +54,7 @@ def _vector(t, name, n, dtype, device):
 
 
 def _call(device, fn, *args):
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)   # current_stream(device).cuda_stream without the object: 0.1 us, not 1.9
     if torch.cuda.current_device() == device.index:
         _lib.check(fn(*args, stream))
     else:

@@ -6,7 +6,7 @@ import ctypes
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, catalogue
 
 
 def _ptr(t):
@@ -274,6 +274,43 @@ class Engine(object):
         with torch.cuda.device(self.device):
             _lib.check(self._L.nncf_predict_scores(self._h, _ptr(uid), p, _ptr(cid), q, _ptr(out), self._stream()))
         return out
+
+    # -- the catalogue head (nncf_amd/catalogue.py) on this engine's tables ----------------
+    def _rows(self, table, ids):
+        out = torch.empty((ids.numel(), self.dim_p), dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(self._L.nncf_gather_rows(_ptr(table), self.dim_p, self.dim_p, _ptr(ids), ids.numel(), 0, _ptr(out), self._stream()))
+        return out
+
+    def softmax_xent(self, uid, cid, weight=None, reduction="mean", grad=True):
+        """Softmax cross entropy of the links (uid, cid) over ALL items -- what the schemes' sampled and shared negatives stand in for --
+        with logits loss_gamma * <u, v> (+ the item's interaction bias), and its gradients: XentResult with d_rows [n, dim] per link,
+        d_table [items, dim] and d_bias.  Nothing is updated.  A negative cid takes its link out.  Rows are used as the tables hold them:
+        an engine that normalises them (emb_normalization) is refused, and so is one whose item table is a text tower's block of a batch."""
+        if self.cfg.normalize_user or self.cfg.normalize_item:
+            raise ValueError("softmax_xent takes rows as they are; this engine normalises them")
+        if getattr(self, "_export", None) is not None:
+            raise ValueError("the item table of this engine is a batch's block of tower outputs, not the catalogue")
+        uid, cid = self.ids(uid), self.ids(cid)
+        if uid.numel() != cid.numel():
+            raise ValueError("%d users, %d items" % (uid.numel(), cid.numel()))
+        bias = self.bias["cb"] if self.bias is not None else None      # a user's bias adds the same to all of its logits
+        return catalogue.softmax_xent(self._rows(self.U, uid)[:, :self.dim], self.V[:, :self.dim], cid, bias=bias, weight=weight,
+                                      scale=self.cfg.loss_gamma, reduction=reduction, grad=grad)
+
+    def quantize_items(self, cid):
+        """The items `cid` in 8 bits (normalised where this engine normalises them), for predict_scores_int8."""
+        return catalogue.quantize_rows(self._rows(self.V, self.ids(cid)), normalize=bool(self.cfg.normalize_item))
+
+    def predict_scores_int8(self, uid, cid, items=None, out=None):
+        """predict_scores from rows in 8 bits: users are quantised on the way in, items are quantize_items(cid) (made here if not given)."""
+        uid, cid = self.ids(uid), self.ids(cid)
+        items = self.quantize_items(cid) if items is None else items
+        users = self._rows(self.U, uid)
+        users = catalogue.quantize_rows(users, normalize=True) if self.cfg.normalize_user else users
+        b = self.bias or {}
+        return catalogue.int8_scores(users, items, row_bias=b["ub"][uid.long()] if b.get("ub") is not None else None,
+                                     col_bias=b["cb"][cid.long()] if b.get("cb") is not None else None, out=out)
 
     def close(self):
         h, self._h = getattr(self, "_h", None), None

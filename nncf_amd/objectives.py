@@ -54,6 +54,9 @@ class Evaluator(object):
         self.user_count = data_spec.user_count
         self.item_count = data_spec.item_count
         self.eval_topk = conf.eval_topk
+        # 'f32' | 'int8': items are ranked by scores of rows held in 8 bits, as a service would that keeps its tables so
+        self.eval_scores = getattr(conf, "eval_scores", "f32")
+        assert self.eval_scores in ("f32", "int8"), "[ERROR] eval_scores %r unknown" % (self.eval_scores,)
         self._dev = None
         self._prepare_for_whole_eval()
 
@@ -87,7 +90,7 @@ class Evaluator(object):
     def _whole(self, model_predict, which, topk, user_chunk=2048, fused=None):
         """test_eval_mat + evaluate_mat (objectives.py:296-370) for one candidate set.  Default: ONE kernel scores and ranks
         (nncf_eval_whole: no (users x candidates) matrix); fused=False (or NNCF_EVAL_FUSED=0, or eval_topk > 100) takes the
-        two-kernel path over a score chunk -- both leave the same bits."""
+        two-kernel path over a score chunk -- both leave the same bits.  eval_scores = 'int8': the two-kernel path on 8-bit scores."""
         predict_engine = getattr(model_predict, "predict_engine", None)
         engine = predict_engine() if predict_engine is not None else model_predict.engine
         st = self._device_state(engine)
@@ -97,7 +100,8 @@ class Evaluator(object):
         metrics, valid = st["metrics"], st["valid"]
         if fused is None:
             fused = os.environ.get("NNCF_EVAL_FUSED", "1") != "0"
-        if fused and topk <= self.FUSED_MAX_TOPK and hasattr(engine, "_h"):
+        int8 = self.eval_scores == "int8"
+        if fused and not int8 and topk <= self.FUSED_MAX_TOPK and hasattr(engine, "_h"):
             with torch.cuda.device(engine.device):
                 stream = _lib.stream_ptr(torch.cuda.current_stream(engine.device))
                 _lib.check(L.nncf_eval_whole(
@@ -108,9 +112,13 @@ class Evaluator(object):
         scores = torch.empty((min(user_chunk, self.user_count), n_cand), dtype=torch.float32, device=engine.device)
         with torch.cuda.device(engine.device):
             stream = _lib.stream_ptr(torch.cuda.current_stream(engine.device))
+            coded = engine.quantize_items(items) if int8 else None
             for u0 in range(0, self.user_count, user_chunk):
                 u1 = min(self.user_count, u0 + user_chunk)
-                model_predict.predict_on_batch_device(st["users"][u0:u1], items, out=scores)
+                if int8:
+                    engine.predict_scores_int8(st["users"][u0:u1], items, items=coded, out=scores[:u1 - u0])
+                else:
+                    model_predict.predict_on_batch_device(st["users"][u0:u1], items, out=scores)
                 _lib.check(L.nncf_eval_topk(
                     ctypes.c_void_p(scores.data_ptr()), u1 - u0, n_cand, n_cand,
                     ctypes.c_void_p(ptr[u0:].data_ptr()), ctypes.c_void_p(idx.data_ptr()), int(topk),
