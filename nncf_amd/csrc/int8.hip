@@ -134,7 +134,7 @@ struct Scores {
 };
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
-// (64 WM) x (64 WC) outputs per workgroup, (32 WM) x (32 WC) per wave, 64 codes a stage, two stages in turn, filled from global memory
+// (64 WM) x (64 WC) outputs per workgroup, (32 WM) x (32 WC) per wave, 64 codes a stage, three stages in turn, filled from global memory
 // without a register (1 KB per wave and instruction: 16 rows of 64 bytes).  Chunks of 16 bytes lie at chunk ^ (row / 4 % 4): the 32 rows
 // of an operand read meet every bank alike.
 typedef const __attribute__((address_space(1))) void* gptr_t;
@@ -147,15 +147,16 @@ struct __attribute__((aligned(16))) CodeStage {
   char x[64 * WM * 64], t[64 * WC * 64];
 };
 
-template <class E, int WM, int WC, bool ONE>
-__global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t c_tiles, int64_t tiles, int vec) {
+template <class E, int WM, int WC>
+__global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t m_tiles, int64_t tiles, int vec) {
   constexpr int MT = 64 * WM, CT = 64 * WC, NX = WM, NT = WC;   // NX + NT fills of 16 rows per wave and stage
-  __shared__ CodeStage<WM, WC> s_a, s_b;
+  __shared__ CodeStage<WM, WC> s_a, s_b, s_c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-  // Workgroups of an XCD (ids of one residue mod 8) take neighbouring tiles of the same rows, so that its L2 sees whole lines of the output
+  // Workgroups of an XCD (ids of one residue mod 8) take neighbouring tiles, all row tiles of a column of tiles after one another: its
+  // L2 reads an eighth of the table and the rows.  (Columns first, every XCD read the whole table: 165 us at 2,000 x 16,384 x 4,096.)
   const int64_t share = (tiles + 7) / 8, tile = (int64_t)(blockIdx.x % 8) * share + blockIdx.x / 8;
   if (tile >= tiles) return;
-  const int64_t m0 = tile / c_tiles * MT, c0 = tile % c_tiles * CT;
+  const int64_t m0 = tile % m_tiles * MT, c0 = tile / m_tiles * CT;
   const int8_t *gx = a.qx + m0 * a.pitch, *gt = a.qt + c0 * a.pitch;
   const int mrows = (int)min((int64_t)MT, a.m - m0), crows = (int)min((int64_t)CT, a.c - c0);
   // rows behind the last are read as the last
@@ -171,10 +172,6 @@ __global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t c
 #pragma unroll
     for (int i = 0; i < NT; ++i) __builtin_amdgcn_global_load_lds((gptr_t)(gt + k0 + ot[i]), (lptr_t)(st.t + (wave * NT + i) * 1024), 16, 0, 0);
     __builtin_amdgcn_sched_barrier(0);   // asked for before the products of the stage, not among them
-  };
-  auto filled = [] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
   };
   const int wm = (wave >> 1) * 32 * WM, wc = (wave & 1) * 32 * WC;
   i32x16 acc[WM][WC];
@@ -198,21 +195,29 @@ __global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t c
 #pragma unroll
         for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[k][i], t[k][j], acc[i][j], 0, 0, 0);
   };
+  // One stage: it has arrived (all but the next one's fills are done) and everyone is done with the one before, whose place the stage after
+  // next takes; then its products.
+  const int stages = (int)(a.pitch / 64);
+  auto step = [&](CodeStage<WM, WC>& now, CodeStage<WM, WC>& after, int k) __attribute__((always_inline)) {
+    // (lgkmcnt: this wave's reads of the stage before have arrived; __syncthreads would wait for the next stage's fills too)
+    if (k + 1 < stages)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NX + NT) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + 2 < stages) fill(after, 64 * (int64_t)(k + 2));
+    work(now);
+  };
   fill(s_a, 0);
-  filled();
-  if constexpr (ONE) {
-    work(s_a);
-    __syncthreads();
-  } else {
-    for (int64_t k0 = 0; k0 < a.pitch; k0 += 128) {   // a pitch above 64 is a multiple of 128
-      fill(s_b, k0 + 64);
-      work(s_a);
-      filled();
-      if (k0 + 128 < a.pitch) fill(s_a, k0 + 128);
-      work(s_b);
-      filled();
-    }
+  if (stages > 1) fill(s_b, 64);
+  int k = 0;
+  for (; k + 3 <= stages; k += 3) {
+    step(s_a, s_c, k);
+    step(s_b, s_a, k + 1);
+    step(s_c, s_b, k + 2);
   }
+  if (k < stages) step(s_a, s_c, k);
+  if (k + 1 < stages) step(s_b, s_a, k + 1);
+  __syncthreads();
   // A wave's 32 x 32 blocks: to rows of 4 adjacent values per lane by way of LDS (8 x 128 bytes per store instruction), where the
   // output allows it.
   float* turn = reinterpret_cast<float*>(s_a.x) + wave * (32 * 40);
@@ -263,6 +268,108 @@ __global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t c
         }
       }
     }
+  }
+}
+
+// ---- many rows of up to 128 codes ----------------------------------------------------------------------------------------------
+// The output is all there is to do: 4 bytes a value against 128 codes.  Its rows start anywhere in a line, and tiles cut at whole columns
+// wrote every 128-byte line that two of them share in parts (16,000 x 16,980 fp32: 370 us, 235 with c = 16,960, whose rows are whole
+// lines).  So a tile computes 256 columns (32 x 256 per wave) and writes, row by row, the 224 that begin with its first whole line; the
+// values go through LDS in a ring of two 32-column blocks, from which each line is taken as soon as its second block is there.
+constexpr int kWideRows = 128, kWideCols = 256, kWideStep = 224;
+
+template <int P>
+__device__ __forceinline__ int wide_at(int row, int chunk) {
+  return P == 128 ? row * 128 + ((chunk ^ (row >> 1 & 7)) << 4) : at64(row, chunk);
+}
+
+template <class E, int P, int VEC>
+__global__ void __launch_bounds__(256, 2) int8_scores_wide_kernel(Scores a, int64_t c_tiles, int64_t tiles) {
+  constexpr int kPitch = 72;      // of the ring, in floats: the two halves of a wave write different banks
+  constexpr int kCodes = (kWideRows + kWideCols) * P, kRing = 4 * 32 * kPitch * 4;
+  __shared__ __attribute__((aligned(16))) char s_mem[kCodes > kRing ? kCodes : kRing];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+  const int64_t share = (tiles + 7) / 8, tile = (int64_t)(blockIdx.x % 8) * share + blockIdx.x / 8;   // neighbours on one XCD
+  if (tile >= tiles) return;
+  const int64_t m0 = tile / c_tiles * kWideRows, c0 = tile % c_tiles * kWideStep;
+  const int mrows = (int)min((int64_t)kWideRows, a.m - m0), crows = (int)min((int64_t)kWideCols, a.c - c0);
+  char *s_x = s_mem, *s_t = s_mem + kWideRows * P;
+  constexpr int kPer = 1024 / P;     // rows of one fill
+  const int frow = lane / (P / 16);
+#pragma unroll
+  for (int i = 0; i < kWideRows / kPer / 4; ++i) {
+    const int r = (i * 4 + wave) * kPer + frow, chunk = (wide_at<P>(r, lane % (P / 16)) >> 4) % (P / 16);
+    __builtin_amdgcn_global_load_lds((gptr_t)(a.qx + (m0 + min(r, mrows - 1)) * P + chunk * 16), (lptr_t)(s_x + (i * 4 + wave) * 1024), 16, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kWideCols / kPer / 4; ++i) {
+    const int r = (i * 4 + wave) * kPer + frow, chunk = (wide_at<P>(r, lane % (P / 16)) >> 4) % (P / 16);
+    __builtin_amdgcn_global_load_lds((gptr_t)(a.qt + (c0 + min(r, crows - 1)) * P + chunk * 16), (lptr_t)(s_t + (i * 4 + wave) * 1024), 16, 0, 0);
+  }
+  const int64_t r0 = m0 + wave * 32;
+  float sx[16], rb[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int64_t row = min(r0 + 8 * (r >> 2) + 4 * half + (r & 3), a.m - 1);
+    sx[r] = a.sx[row];
+    rb[r] = a.rb ? a.rb[row] : 0.f;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  i32x16 acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0;
+#pragma unroll
+  for (int k = 0; k < P / 32; ++k) {
+    const i32x4 x = *reinterpret_cast<const i32x4*>(s_x + wide_at<P>(wave * 32 + col, 2 * k + half));
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x, *reinterpret_cast<const i32x4*>(s_t + wide_at<P>(32 * j + col, 2 * k + half)), acc[j], 0, 0, 0);
+  }
+  __syncthreads();
+  float* ring = reinterpret_cast<float*>(s_mem) + wave * (32 * kPitch);
+  const uint32_t phase = (uint32_t)((uintptr_t)a.out / sizeof(E) + c0);      // of a row's first value, with its row's offset, mod 32
+  constexpr int kLanes = 32 / VEC, kRowsPer = 64 / kLanes, kTurns = 32 / kRowsPer;
+  const int in = lane / kLanes, e0 = lane % kLanes * VEC;
+  auto emit = [&](int line) __attribute__((always_inline)) {
+#pragma unroll 4
+    for (int q = 0; q < kTurns; ++q) {
+      const int r = kRowsPer * q + in;
+      const int64_t row = r0 + r;
+      const int first = (int)(-(phase + (uint32_t)row * (uint32_t)a.out_stride) & 31);   // columns before the first whole line
+      const int x = first + 32 * line + e0;
+      if (row < a.m && x >= 0 && c0 + x < a.c) {
+        E* dst = reinterpret_cast<E*>(a.out) + row * a.out_stride + c0 + x;
+        if constexpr (VEC == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(ring + r * kPitch + (x & 63));
+          typedef E E4 __attribute__((ext_vector_type(4)));
+          E4 o;
+          o[0] = (E)f.x;
+          o[1] = (E)f.y;
+          o[2] = (E)f.z;
+          o[3] = (E)f.w;
+          *reinterpret_cast<E4*>(dst) = o;
+        } else {
+          *dst = (E)ring[r * kPitch + (x & 63)];
+        }
+      }
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    __builtin_amdgcn_sched_barrier(0);   // block by block: the next one's scales would take the registers of its sums
+    const int64_t item = min(c0 + 32 * j + col, a.c - 1);
+    const float st = a.st[item], cb = a.cb ? a.cb[item] : 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      ring[(8 * (r >> 2) + 4 * half + (r & 3)) * kPitch + (j & 1) * 32 + col] = ((float)acc[j][r] * sx[r]) * st + (rb[r] + cb);
+    __builtin_amdgcn_wave_barrier();
+    if (j == 0) {
+      if (c0 == 0) emit(-1);
+    } else {
+      emit(j - 1);
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -377,10 +484,7 @@ int run_many(const Scores& a, hipStream_t st) {
   const int vec = a.c % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(E)) == 0;
   ProfScope ps("int8_scores_kernel", st);
   const dim3 grid((unsigned)((mt * ct + 7) / 8 * 8));
-  if (a.pitch == 64)
-    hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC, true>), grid, dim3(256), 0, st, a, ct, mt * ct, vec);
-  else
-    hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC, false>), grid, dim3(256), 0, st, a, ct, mt * ct, vec);
+  hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC>), grid, dim3(256), 0, st, a, mt, mt * ct, vec);
   NNCF_HIP_CHECK(hipGetLastError());
   return NNCF_OK;
 }
@@ -388,6 +492,23 @@ int run_many(const Scores& a, hipStream_t st) {
 template <class E>
 int run_scores(const Scores& a, hipStream_t st) {
   if (a.m <= 32) return run_few<E, float, false>(a, FloatRows{}, st);
+  const int64_t wide_c = (a.c + kWideStep - 1) / kWideStep, wide = (a.m + kWideRows - 1) / kWideRows * wide_c;
+  if (a.pitch <= 128 && wide >= 256) {
+    NNCF_REQUIRE(wide < (1LL << 30), "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
+    const bool vec = a.c % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(E)) == 0;
+    const dim3 grid((unsigned)((wide + 7) / 8 * 8));
+    ProfScope ps("int8_scores_kernel", st);
+    if (a.pitch == 64 && vec)
+      hipLaunchKernelGGL((int8_scores_wide_kernel<E, 64, 4>), grid, dim3(256), 0, st, a, wide_c, wide);
+    else if (a.pitch == 64)
+      hipLaunchKernelGGL((int8_scores_wide_kernel<E, 64, 1>), grid, dim3(256), 0, st, a, wide_c, wide);
+    else if (vec)
+      hipLaunchKernelGGL((int8_scores_wide_kernel<E, 128, 4>), grid, dim3(256), 0, st, a, wide_c, wide);
+    else
+      hipLaunchKernelGGL((int8_scores_wide_kernel<E, 128, 1>), grid, dim3(256), 0, st, a, wide_c, wide);
+    NNCF_HIP_CHECK(hipGetLastError());
+    return NNCF_OK;
+  }
   // large tiles once they are enough for every CU
   const int64_t large = (a.m + 127) / 128 * ((a.c + 255) / 256);
   return large >= 256 ? run_many<E, 2, 4>(a, st) : run_many<E, 1, 1>(a, st);

@@ -308,6 +308,24 @@ def test_scores(m, c, k, dtype):
     assert torch.equal(got, catalogue.int8_scores(catalogue.quantize_rows(x), table, dtype=dtype, **kw))
 
 
+@pytest.mark.parametrize("m,c,k,pad,off", [(1000, 8001, 100, 0, 0), (4100, 2000, 50, 0, 0), (2050, 4100, 128, 4, 4), (2000, 3999, 64, 30, 13),
+                                           (3000, 2244, 20, 0, 0), (300, 30000, 100, 0, 0), (3000, 2200, 300, 0, 0)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_scores_of_many_rows(m, c, k, pad, off, dtype):
+    """Launches of many workgroups: rows that start anywhere in a line, in rows of a wider matrix, whose other columns stay."""
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x, t = catalogue.quantize_rows(torch.randn(m, k, generator=g, device=DEV)), catalogue.quantize_rows(torch.randn(c, k, generator=g, device=DEV))
+    rb, cb = torch.randn(m, generator=g, device=DEV), torch.randn(c, generator=g, device=DEV)
+    wide = torch.full((m, c + pad + off), 7.0, device=DEV, dtype=dtype)
+    out = wide[:, off:off + c]
+    catalogue.int8_scores(x, t, row_bias=rb, col_bias=cb, out=out)
+    exact = (x.codes[:, :k].double() @ t.codes[:, :k].double().t()) * x.scale[:, None].double() * t.scale[None].double()
+    want = exact + rb[:, None].double() + cb[None].double()
+    tol = 5 * 2.0 ** -24 * (exact.abs() + rb.abs()[:, None] + cb.abs()[None]) + U[dtype] * want.abs() + (2.0 ** -25 if dtype == F16 else 1e-30)
+    assert ((out.double() - want).abs() <= tol).all()
+    assert (wide[:, :off] == 7).all() and (wide[:, off + c:] == 7).all()
+
+
 @pytest.mark.parametrize("m", [3, 40])
 def test_scores_write_only_their_columns(m):
     x, t = torch.randn(m, 30, device=DEV), torch.randn(45, 30, device=DEV)
