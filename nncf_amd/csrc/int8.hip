@@ -134,26 +134,32 @@ struct Scores {
 };
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
-// (64 WM) x (64 WC) outputs per workgroup, (32 WM) x (32 WC) per wave, 64 codes a stage, three stages in turn, filled from global memory
-// without a register (1 KB per wave and instruction: 16 rows of 64 bytes).  Chunks of 16 bytes lie at chunk ^ (row / 4 % 4): the 32 rows
-// of an operand read meet every bank alike.
+// (32 WM) x (32 WC) outputs per wave, RW x 2 waves; KB codes of every row a stage, two stages in turn, filled from global memory without a
+// register (1 KB per wave and instruction).  Chunks of 16 bytes are placed so that the 32 rows of an operand read meet every bank alike.
+// 128 codes a stage are whole lines: in halves, the tile of 128 x 256 took 165 us at 2,000 x 16,384 x 4,096, whatever lay ahead (two
+// stages or three) -- 22 bytes a cycle and CU, as halves of lines.
 typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 
-__device__ __forceinline__ int at64(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 2 & 3)) << 4); }
+template <int KB>
+__device__ __forceinline__ int code_at(int row, int chunk) {
+  return KB == 128 ? row * 128 + ((chunk ^ (row >> 1 & 7)) << 4) : row * 64 + ((chunk ^ (row >> 2 & 3)) << 4);
+}
 
-template <int WM, int WC>
+template <int XR, int TR, int KB>
 struct __attribute__((aligned(16))) CodeStage {
-  char x[64 * WM * 64], t[64 * WC * 64];
+  char x[XR * KB], t[TR * KB];
 };
 
-template <class E, int WM, int WC>
-__global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t m_tiles, int64_t tiles, int vec) {
-  constexpr int MT = 64 * WM, CT = 64 * WC, NX = WM, NT = WC;   // NX + NT fills of 16 rows per wave and stage
-  __shared__ CodeStage<WM, WC> s_a, s_b, s_c;
+template <class E, int WM, int WC, int RW, int KB>
+__global__ void __launch_bounds__(128 * RW, 2) int8_scores_kernel(Scores a, int64_t m_tiles, int64_t tiles, int vec) {
+  constexpr int MT = 32 * WM * RW, CT = 64 * WC, kPer = 1024 / KB;   // kPer rows of one fill
+  constexpr int NX = MT / kPer / (2 * RW), NT = CT / kPer / (2 * RW);
+  typedef CodeStage<MT, CT, KB> Stage;
+  __shared__ Stage s_a, s_b;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   // Workgroups of an XCD (ids of one residue mod 8) take neighbouring tiles, all row tiles of a column of tiles after one another: its
-  // L2 reads an eighth of the table and the rows.  (Columns first, every XCD read the whole table: 165 us at 2,000 x 16,384 x 4,096.)
+  // L2 reads an eighth of the table and the rows.
   const int64_t share = (tiles + 7) / 8, tile = (int64_t)(blockIdx.x % 8) * share + blockIdx.x / 8;
   if (tile >= tiles) return;
   const int64_t m0 = tile % m_tiles * MT, c0 = tile / m_tiles * CT;
@@ -161,67 +167,68 @@ __global__ void __launch_bounds__(256, 2) int8_scores_kernel(Scores a, int64_t m
   const int mrows = (int)min((int64_t)MT, a.m - m0), crows = (int)min((int64_t)CT, a.c - c0);
   // rows behind the last are read as the last
   uint32_t ox[NX], ot[NT];
-  const int frow = lane >> 2, fchunk = ((lane & 3) ^ (lane >> 4 & 3)) << 4;
+  const int frow = lane / (KB / 16);
 #pragma unroll
-  for (int i = 0; i < NX; ++i) ox[i] = (uint32_t)min((wave * NX + i) * 16 + frow, mrows - 1) * (uint32_t)a.pitch + fchunk;
+  for (int i = 0; i < NX; ++i) {
+    const int r = (wave * NX + i) * kPer + frow;
+    ox[i] = (uint32_t)min(r, mrows - 1) * (uint32_t)a.pitch + code_at<KB>(r, lane % (KB / 16)) % KB;
+  }
 #pragma unroll
-  for (int i = 0; i < NT; ++i) ot[i] = (uint32_t)min((wave * NT + i) * 16 + frow, crows - 1) * (uint32_t)a.pitch + fchunk;
-  auto fill = [&](CodeStage<WM, WC>& st, int64_t k0) __attribute__((always_inline)) {
+  for (int i = 0; i < NT; ++i) {
+    const int r = (wave * NT + i) * kPer + frow;
+    ot[i] = (uint32_t)min(r, crows - 1) * (uint32_t)a.pitch + code_at<KB>(r, lane % (KB / 16)) % KB;
+  }
+  auto fill = [&](Stage& st, int64_t k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NX; ++i) __builtin_amdgcn_global_load_lds((gptr_t)(gx + k0 + ox[i]), (lptr_t)(st.x + (wave * NX + i) * 1024), 16, 0, 0);
 #pragma unroll
     for (int i = 0; i < NT; ++i) __builtin_amdgcn_global_load_lds((gptr_t)(gt + k0 + ot[i]), (lptr_t)(st.t + (wave * NT + i) * 1024), 16, 0, 0);
     __builtin_amdgcn_sched_barrier(0);   // asked for before the products of the stage, not among them
   };
-  const int wm = (wave >> 1) * 32 * WM, wc = (wave & 1) * 32 * WC;
+  auto filled = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  const int wm = (wave >> 1) * 32 * WM, wc = (wave & 1) * 32 * WC;   // of RW x 2 waves
   i32x16 acc[WM][WC];
 #pragma unroll
   for (int i = 0; i < WM; ++i)
 #pragma unroll
     for (int j = 0; j < WC; ++j) acc[i][j] = 0;
-  auto work = [&](const CodeStage<WM, WC>& st) __attribute__((always_inline)) {
-    i32x4 x[2][WM], t[2][WC];
+  auto work = [&](const Stage& st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < KB / 32; ++k) {
+      i32x4 x[WM], t[WC];
 #pragma unroll
-      for (int i = 0; i < WM; ++i) x[k][i] = *reinterpret_cast<const i32x4*>(st.x + at64(wm + 32 * i + col, 2 * k + half));
+      for (int i = 0; i < WM; ++i) x[i] = *reinterpret_cast<const i32x4*>(st.x + code_at<KB>(wm + 32 * i + col, 2 * k + half));
 #pragma unroll
-      for (int j = 0; j < WC; ++j) t[k][j] = *reinterpret_cast<const i32x4*>(st.t + at64(wc + 32 * j + col, 2 * k + half));
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int j = 0; j < WC; ++j) t[j] = *reinterpret_cast<const i32x4*>(st.t + code_at<KB>(wc + 32 * j + col, 2 * k + half));
 #pragma unroll
       for (int j = 0; j < WC; ++j)
 #pragma unroll
-        for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[k][i], t[k][j], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], t[j], acc[i][j], 0, 0, 0);
+    }
   };
-  // One stage: it has arrived (all but the next one's fills are done) and everyone is done with the one before, whose place the stage after
-  // next takes; then its products.
-  const int stages = (int)(a.pitch / 64);
-  auto step = [&](CodeStage<WM, WC>& now, CodeStage<WM, WC>& after, int k) __attribute__((always_inline)) {
-    // (lgkmcnt: this wave's reads of the stage before have arrived; __syncthreads would wait for the next stage's fills too)
-    if (k + 1 < stages)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NX + NT) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (k + 2 < stages) fill(after, 64 * (int64_t)(k + 2));
-    work(now);
-  };
+  const int stages = (int)(a.pitch / KB);
   fill(s_a, 0);
-  if (stages > 1) fill(s_b, 64);
+  filled();
   int k = 0;
-  for (; k + 3 <= stages; k += 3) {
-    step(s_a, s_c, k);
-    step(s_b, s_a, k + 1);
-    step(s_c, s_b, k + 2);
+  for (; k + 2 <= stages; k += 2) {
+    fill(s_b, (int64_t)(k + 1) * KB);
+    work(s_a);
+    filled();
+    if (k + 2 < stages) fill(s_a, (int64_t)(k + 2) * KB);
+    work(s_b);
+    filled();
   }
-  if (k < stages) step(s_a, s_c, k);
-  if (k + 1 < stages) step(s_b, s_a, k + 1);
-  __syncthreads();
+  if (k < stages) {
+    work(s_a);
+    __syncthreads();
+  }
   // A wave's 32 x 32 blocks: to rows of 4 adjacent values per lane by way of LDS (8 x 128 bytes per store instruction), where the
   // output allows it.
   float* turn = reinterpret_cast<float*>(s_a.x) + wave * (32 * 40);
-  static_assert(sizeof(s_a) >= 4 * 32 * 40 * 4 || WM * WC == 1, "room to turn a block per wave");
+  static_assert(sizeof(s_a) >= 2 * RW * 32 * 40 * 4 || WM * WC == 1, "room to turn a block per wave");
 #pragma unroll
   for (int i = 0; i < WM; ++i) {
     float sx[16], rb[16];
@@ -280,7 +287,7 @@ constexpr int kWideRows = 128, kWideCols = 256, kWideStep = 224;
 
 template <int P>
 __device__ __forceinline__ int wide_at(int row, int chunk) {
-  return P == 128 ? row * 128 + ((chunk ^ (row >> 1 & 7)) << 4) : at64(row, chunk);
+  return code_at<P>(row, chunk);
 }
 
 template <class E, int P, int VEC>
@@ -477,14 +484,14 @@ int run_few(const Scores& a, const FloatRows& f, hipStream_t st) {
   return NNCF_OK;
 }
 
-template <class E, int WM, int WC>
+template <class E, int WM, int WC, int RW, int KB>
 int run_many(const Scores& a, hipStream_t st) {
-  const int64_t mt = (a.m + 64 * WM - 1) / (64 * WM), ct = (a.c + 64 * WC - 1) / (64 * WC);
+  const int64_t mt = (a.m + 32 * WM * RW - 1) / (32 * WM * RW), ct = (a.c + 64 * WC - 1) / (64 * WC);
   NNCF_REQUIRE(mt * ct < (1LL << 30), "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
   const int vec = a.c % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(E)) == 0;
-  ProfScope ps("int8_scores_kernel", st);
   const dim3 grid((unsigned)((mt * ct + 7) / 8 * 8));
-  hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC>), grid, dim3(256), 0, st, a, mt, mt * ct, vec);
+  ProfScope ps("int8_scores_kernel", st);
+  hipLaunchKernelGGL((int8_scores_kernel<E, WM, WC, RW, KB>), grid, dim3(128 * RW), 0, st, a, mt, mt * ct, vec);
   NNCF_HIP_CHECK(hipGetLastError());
   return NNCF_OK;
 }
@@ -510,8 +517,8 @@ int run_scores(const Scores& a, hipStream_t st) {
     return NNCF_OK;
   }
   // large tiles once they are enough for every CU
-  const int64_t large = (a.m + 127) / 128 * ((a.c + 255) / 256);
-  return large >= 256 ? run_many<E, 2, 4>(a, st) : run_many<E, 1, 1>(a, st);
+  const int64_t large = (a.m + 255) / 256 * ((a.c + 255) / 256);
+  return large >= 256 && a.pitch >= 128 ? run_many<E, 2, 4, 4, 128>(a, st) : run_many<E, 1, 1, 2, 64>(a, st);
 }
 
 template <class E>
