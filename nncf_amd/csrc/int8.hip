@@ -208,6 +208,20 @@ __global__ void __launch_bounds__(128 * RW, 2) int8_scores_kernel(Scores a, int6
 #pragma unroll
         for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], t[j], acc[i][j], 0, 0, 0);
     }
+    // one step's operands are read among the products of the step before
+    if (WM * WC > 1) {
+      __builtin_amdgcn_sched_group_barrier(0x100, WM + WC, 0);
+#pragma unroll
+      for (int k = 1; k < KB / 32; ++k) {
+#pragma unroll
+        for (int i = 0; i < WM + WC; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, WM * WC - WM - WC, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, WM * WC, 0);
+    }
   };
   const int stages = (int)(a.pitch / KB);
   fill(s_a, 0);
