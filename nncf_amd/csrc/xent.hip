@@ -510,6 +510,12 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, 
 }
 
 // ---- joining the splits ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int rows_with_target(const int32_t* target, int n) {
+  int k = 0;
+  for (int i = 0; i < n; ++i) k += target[i] >= 0;
+  return k;
+}
+
 struct RowsOut {
   const void *rows, *table;
   int64_t rows_stride, table_stride;
@@ -595,7 +601,7 @@ __global__ void __launch_bounds__(256) xent_rows_kernel(RowsOut a, Part part) {
   if (!has) {
     each = lse = q = w = 0.f;
   }
-  const float g = a.mean ? w / (float)max(1, *a.valid) : w;
+  const float g = a.mean ? w / (float)max(1, a.valid ? *a.valid : rows_with_target(a.target, (int)a.n)) : w;
   if (lane == 0) {
     // a weight of zero takes the row out of the loss, whatever its loss is
     a.loss_rows[row] = has && !(w == 0.f) ? w * each : 0.f;
@@ -647,6 +653,202 @@ __device__ __forceinline__ void total_loss(const float* rows, int64_t n, int mea
 }
 
 __global__ void __launch_bounds__(256) xent_loss_kernel(TableOut a) { total_loss(a.loss_rows, a.n, a.mean, a.valid, a.loss); }
+
+// ---- a few rows --------------------------------------------------------------------------------------------------------------
+// Up to N rows live in the registers of every 16-lane group (8 columns a lane); a group takes an item's row as it lies in the table, four
+// items at a time, in fp32: no image, no matrix instruction, and the table's bytes are the bound.
+struct Few {
+  const void *rows, *table;
+  int64_t rows_stride, table_stride;
+  const int32_t* target;
+  const float *bias, *h, *kq, *sgn;
+  int64_t c, per;      // items of a workgroup
+  float scale;
+  int n, d, rows_vec, table_vec, out_vec;
+  // backward
+  const float* loss_rows;
+  float* loss;
+  void* d_table;
+  float* d_bias;
+  int mean, reduce;
+};
+template <class E, int N>
+__device__ __forceinline__ void load_few(const Few& a, int q, float (&u)[N][8], int32_t (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = i < a.n ? a.target[i] : -1;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[i][e] = 0.f;
+    if (t[i] >= 0) load8(reinterpret_cast<const E*>(a.rows) + i * a.rows_stride, 8 * q, a.d, a.rows_vec != 0, u[i]);
+  }
+}
+// base-2 logits of an item against the rows, in every lane of the group
+template <int N>
+__device__ __forceinline__ void few_logits(const float (&u)[N][8], const float (&v)[8], float scale2, float b2, float (&y)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(u[i][e], v[e], s);
+    y[i] = fmaf(row16_sum(s), scale2, b2);
+  }
+}
+
+template <class E, int N, bool MEAN>
+__global__ void __launch_bounds__(256) xent_few_forward_kernel(Few a, Part part, int64_t rows_pad) {
+  __shared__ float s_m[16][N], s_l[16][N], s_o[MEAN ? 16 : 1][MEAN ? 128 : 1];
+  const int q = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const float scale2 = a.scale * kLog2e;
+  float u[N][8], m[N], l[N], o[MEAN ? N : 1][8];
+  int32_t t[N];
+  load_few<E, N>(a, q, u, t);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (MEAN) o[i][e] = 0.f;
+  }
+  const int64_t end = min(a.c, (int64_t)(blockIdx.x + 1) * a.per);
+  for (int64_t j0 = (int64_t)blockIdx.x * a.per + group; j0 < end; j0 += 64) {
+    float v[4][8], b2[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t j = j0 + 16 * k;
+      b2[k] = j < end ? (a.bias ? a.bias[j] * kLog2e : 0.f) : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+      if (!(b2[k] == -INFINITY)) load8(reinterpret_cast<const E*>(a.table) + j * a.table_stride, 8 * q, a.d, a.table_vec != 0, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float y[N];
+      few_logits<N>(u, v[k], scale2, b2[k], y);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float z = j0 + 16 * k == t[i] ? -INFINITY : y[i];
+        const float to = fmaxf(m[i], z != z ? 0.f : z);     // a NaN has to reach the sums
+        if (!(to == -INFINITY)) {
+          const float f = __builtin_amdgcn_exp2f(m[i] - to), p = __builtin_amdgcn_exp2f(z - to);
+          m[i] = to;
+          l[i] = fmaf(l[i], f, p);
+          if (MEAN) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[i][e] = fmaf(o[i][e], f, p * v[k][e]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (q == 0) {
+      s_m[group][i] = m[i];
+      s_l[group][i] = l[i];
+    }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= a.n) break;
+    float top = -INFINITY;
+    for (int g = 0; g < 16; ++g) top = fmaxf(top, s_m[g][i]);
+    const bool some = top > -INFINITY;
+    const int64_t at = (int64_t)blockIdx.x * rows_pad + i;
+    if (MEAN) {
+      const float f = some && m[i] > -INFINITY ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_o[group][8 * q + e] = f == 0.f ? 0.f : o[i][e] * f;
+      __syncthreads();
+      if (threadIdx.x < 128) {
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) sum += s_o[g][threadIdx.x];
+        part.o[at * 128 + threadIdx.x] = sum;
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      float sum = 0.f;
+      for (int g = 0; g < 16; ++g)
+        if (some && s_m[g][i] > -INFINITY) sum += s_l[g][i] * __builtin_amdgcn_exp2f(s_m[g][i] - top);
+      part.m[at] = top;
+      part.l[at] = sum;
+    }
+  }
+}
+
+template <class E, int N>
+__global__ void __launch_bounds__(256) xent_few_backward_kernel(Few a) {
+  if (a.reduce && blockIdx.x == gridDim.x - 1) {
+    const int32_t has = rows_with_target(a.target, a.n);
+    total_loss(a.loss_rows, a.n, a.mean, &has, a.loss);
+    return;
+  }
+  const int q = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const float scale2 = a.scale * kLog2e;
+  const float share = a.mean ? 1.f / (float)max(1, rows_with_target(a.target, a.n)) : 1.f;
+  float u[N][8], h[N], kq[N], sg[N];
+  int32_t t[N];
+  load_few<E, N>(a, q, u, t);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool in = i < a.n;
+    h[i] = in ? a.h[i] : -INFINITY;
+    kq[i] = in ? a.kq[i] : 0.f;
+    sg[i] = in ? a.sgn[i] : 1.f;
+  }
+  const int64_t end = min(a.c, (int64_t)(blockIdx.x + 1) * a.per);
+  for (int64_t j0 = (int64_t)blockIdx.x * a.per + group; j0 < end; j0 += 64) {
+    float v[4][8], b2[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t j = j0 + 16 * k;
+      b2[k] = j < end ? (a.bias ? a.bias[j] * kLog2e : 0.f) : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+      if (!(b2[k] == -INFINITY)) load8(reinterpret_cast<const E*>(a.table) + j * a.table_stride, 8 * q, a.d, a.table_vec != 0, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t j = j0 + 16 * k;
+      if (j >= end) break;
+      const bool out = b2[k] == -INFINITY;
+      float y[N], x[8] = {}, sum = 0.f;
+      few_logits<N>(u, v[k], scale2, b2[k], y);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float w = out ? 0.f : j == t[i] ? -kq[i] : sg[i] * __builtin_amdgcn_exp2f(y[i] + h[i]);
+        sum += w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(w, u[i][e], x[e]);
+      }
+      E* dst = reinterpret_cast<E*>(a.d_table) + j * a.d + 8 * q;
+      const float s = a.scale * share;
+      if (a.out_vec) {
+        typedef E E4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (8 * q + 4 * g < a.d) {
+            E4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (E)(x[4 * g + e] * s);
+            *reinterpret_cast<E4*>(dst + 4 * g) = o;
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * q + e < a.d) dst[e] = (E)(x[e] * s);
+      }
+      if (q == 0 && a.d_bias) a.d_bias[j] = sum * share;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) xent_few_loss_kernel(Few a) {
+  const int32_t has = rows_with_target(a.target, a.n);
+  total_loss(a.loss_rows, a.n, a.mean, &has, a.loss);
+}
 
 // One row of the table per DP / 4 lanes: joins its splits, applies the scales; the last workgroup sums the losses.
 template <class E, int DP>
@@ -748,6 +950,9 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
   return y;
 }
 
+// Up to kFewRows rows: see xent_few_forward_kernel.
+constexpr int kFewRows = 4, kFewSplits = 256;
+
 template <class T, int NP, int DP>
 int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
   typedef typename std::conditional<NP == 2, float, typename T::E>::type E;
@@ -815,6 +1020,73 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
   return NNCF_OK;
 }
 
+struct FewLayout {
+  int splits;
+  int64_t per, o, m, l, h, kq, sgn, loss, bytes;
+};
+FewLayout few_layout(int64_t n, int64_t c, bool grad) {
+  FewLayout y{};
+  y.per = up((c + kFewSplits - 1) / kFewSplits, 64);
+  y.splits = (int)((c + y.per - 1) / y.per);
+  int64_t at = 0;
+  auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };
+  y.o = take(grad ? (int64_t)y.splits * kFewRows * 128 * 4 : 0);
+  y.m = take((int64_t)y.splits * kFewRows * 4);
+  y.l = take((int64_t)y.splits * kFewRows * 4);
+  y.h = take(kFewRows * 4);
+  y.kq = take(kFewRows * 4);
+  y.sgn = take(kFewRows * 4);
+  y.loss = take(kFewRows * 4);
+  y.bytes = at;
+  return y;
+}
+
+template <class E, int N>
+int run_few(const nncf_xent* x, char* ws, hipStream_t st) {
+  const bool grad = x->d_rows != nullptr;
+  const FewLayout y = few_layout(x->n, x->c, grad);
+  auto f = [ws](int64_t at) { return reinterpret_cast<float*>(ws + at); };
+  auto vec = [](const void* p, int64_t stride) { return ((uintptr_t)p % (4 * sizeof(E)) == 0 && stride % 4 == 0) ? 1 : 0; };
+  const bool scalar = x->reduction != NNCF_NONE;
+  const int mean = x->reduction == NNCF_MEAN;
+  float* loss_rows = scalar ? f(y.loss) : x->loss;
+  const Few a{x->rows, x->table, x->rows_stride, x->table_stride, x->target, x->bias, f(y.h), f(y.kq), f(y.sgn), x->c, y.per, x->scale, (int)x->n,
+              x->dim, vec(x->rows, x->rows_stride), vec(x->table, x->table_stride), vec(x->d_table, x->dim), loss_rows, x->loss, x->d_table, x->d_bias, mean, scalar};
+  const Part part{f(y.o), f(y.m), f(y.l)};
+  const RowsOut ro{x->rows, x->table, x->rows_stride, x->table_stride, x->bias, x->weight, x->target, nullptr, loss_rows, x->lse,
+                   grad ? f(y.h) : nullptr, f(y.kq), f(y.sgn), nullptr, x->d_rows, x->scale, x->n, x->c, kFewRows, x->dim, mean, y.splits};
+  {
+    ProfScope ps("xent_few_forward_kernel", st);
+    if (grad)
+      hipLaunchKernelGGL((xent_few_forward_kernel<E, N, true>), dim3((unsigned)y.splits), dim3(256), 0, st, a, part, (int64_t)kFewRows);
+    else
+      hipLaunchKernelGGL((xent_few_forward_kernel<E, N, false>), dim3((unsigned)y.splits), dim3(256), 0, st, a, part, (int64_t)kFewRows);
+  }
+  {
+    ProfScope ps("xent_rows_kernel", st);
+    if (grad)
+      hipLaunchKernelGGL((xent_rows_kernel<E, 1, 128, true, 4>), dim3((unsigned)x->n), dim3(256), 0, st, ro, part);
+    else
+      hipLaunchKernelGGL((xent_rows_kernel<E, 1, 128, false, 1>), dim3((unsigned)((x->n + 3) / 4)), dim3(256), 0, st, ro, part);
+  }
+  if (grad) {
+    ProfScope ps("xent_few_backward_kernel", st);
+    Few b = a;
+    b.per = up((x->c + 2047) / 2048, 64);      // as many workgroups as the device holds: nothing is joined behind them
+    hipLaunchKernelGGL((xent_few_backward_kernel<E, N>), dim3((unsigned)((x->c + b.per - 1) / b.per + (scalar ? 1 : 0))), dim3(256), 0, st, b);
+  } else if (scalar) {
+    hipLaunchKernelGGL((xent_few_loss_kernel), dim3(1), dim3(256), 0, st, a);
+  }
+  NNCF_HIP_CHECK(hipGetLastError());
+  return NNCF_OK;
+}
+
+template <class E>
+int run_few_rows(const nncf_xent* x, char* ws, hipStream_t st) {
+  if (x->n == 1) return run_few<E, 1>(x, ws, st);
+  return run_few<E, 4>(x, ws, st);
+}
+
 int check_shape(int64_t n, int64_t c, int32_t dim, int32_t dtype) {
   NNCF_REQUIRE(n > 0 && n <= (int64_t)kOwn * 65535, "n = %lld rows out of range (1..%lld)", (long long)n, (long long)kOwn * 65535);
   // own tiles of a launch are its grid's second dimension
@@ -828,6 +1100,7 @@ int check_shape(int64_t n, int64_t c, int32_t dim, int32_t dtype) {
 
 extern "C" int64_t nncf_softmax_xent_ws_bytes(int64_t n, int64_t c, int32_t dim, int32_t dtype, int32_t with_grad) {
   if (nncf::check_shape(n, c, dim, dtype) != NNCF_OK) return -1;
+  if (n <= nncf::kFewRows) return nncf::few_layout(n, c, with_grad != 0).bytes;
   return nncf::layout(n, c, dim, dtype, with_grad != 0).bytes;
 }
 
@@ -845,11 +1118,18 @@ extern "C" int nncf_softmax_xent(const nncf_xent* x, void* d_ws, int64_t ws_byte
   const uintptr_t es = x->dtype == NNCF_F32 ? 4 : 2;
   NNCF_REQUIRE((uintptr_t)x->rows % es == 0 && (uintptr_t)x->table % es == 0 && (uintptr_t)x->d_rows % es == 0 &&
                (uintptr_t)x->d_table % es == 0, "a tensor is not aligned to its elements");
-  const Layout y = layout(x->n, x->c, x->dim, x->dtype, x->d_rows != nullptr);
-  NNCF_REQUIRE(ws_bytes >= y.bytes, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)y.bytes);
+  const bool few = x->n <= kFewRows;
+  const Layout y = few ? Layout{} : layout(x->n, x->c, x->dim, x->dtype, x->d_rows != nullptr);
+  const int64_t need = few ? few_layout(x->n, x->c, x->d_rows != nullptr).bytes : y.bytes;
+  NNCF_REQUIRE(ws_bytes >= need, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
   NNCF_REQUIRE(((uintptr_t)d_ws & 255) == 0, "workspace must be 256-byte aligned");
   char* ws = reinterpret_cast<char*>(d_ws);
   hipStream_t st = as_stream(stream);
+  if (few) {
+    if (x->dtype == NNCF_F32) return run_few_rows<float>(x, ws, st);
+    if (x->dtype == NNCF_F16) return run_few_rows<_Float16>(x, ws, st);
+    return run_few_rows<__bf16>(x, ws, st);
+  }
   const bool wide = y.dp == 128;
   if (x->dtype == NNCF_F32) return wide ? run<F16, 2, 128>(x, y, ws, st) : run<F16, 2, 64>(x, y, ws, st);
   if (x->dtype == NNCF_F16) return wide ? run<F16, 1, 128>(x, y, ws, st) : run<F16, 1, 64>(x, y, ws, st);
