@@ -413,6 +413,17 @@ __global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRow
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int8_t* qx = a.qx;
   const float* sx = a.sx;
+  // the table's first 128 codes are asked for before anything else
+  const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * 128;
+  const int8_t* t[4];
+  i32x4 ahead[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    t[j] = a.qt + min(first + 32 * j + col, a.c - 1) * a.pitch + half * 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < 2 || a.pitch > 64) ahead[j][k] = *reinterpret_cast<const i32x4*>(t[j] + 32 * k);
+  }
   if constexpr (FUSED) {
     for (int r = wave; r < a.m; r += 4) {
       const X* src = reinterpret_cast<const X*>(f.x) + r * f.stride;
@@ -444,16 +455,18 @@ __global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRow
     sx = s_sx;
   }
   const int8_t* x = qx + min((int64_t)col, a.m - 1) * a.pitch + half * 16;
-  const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * 128;
   if (first >= a.c) return;
-  const int8_t* t[4];
   i32x16 acc[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    t[j] = a.qt + min(first + 32 * j + col, a.c - 1) * a.pitch + half * 16;
-    acc[j] = 0;
-  }
-  for (int64_t k0 = 0; k0 < a.pitch; k0 += 64) {
+  for (int j = 0; j < 4; ++j) acc[j] = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < 2 || a.pitch > 64) {
+      const i32x4 xk = *reinterpret_cast<const i32x4*>(x + 32 * k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xk, ahead[j][k], acc[j], 0, 0, 0);
+    }
+  for (int64_t k0 = 128; k0 < a.pitch; k0 += 64) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const i32x4 xk = *reinterpret_cast<const i32x4*>(x + k0 + 32 * k);

@@ -61,6 +61,14 @@ struct Side {
   int64_t rows;       // rows of the call
   int64_t rows_pad;   // a multiple of 128
 };
+// Where a pass over items that are not split puts its results: the gradients themselves (table NULL: Part).
+struct Grad {
+  void* table;
+  float* bias;
+  const int32_t* valid;
+  float scale;
+  int d, mean, vec;
+};
 struct Part {   // results of the streaming kernel: [splits][own rows_pad]
   float *o, *m, *l;
 };
@@ -157,7 +165,7 @@ __device__ __forceinline__ typename T::V read_cols(const char* lds, int plane, i
 
 // The streaming kernel.  BWD: own rows are items.  WT: row weights of either sign.  MEAN: the O sums are wanted.
 template <class T, int NP, int DP, bool BWD, bool WT, bool MEAN>
-__global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str, Part part, float scale2, int stages, int stages_per_split) {
+__global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str, Part part, Grad grad, float scale2, int stages, int stages_per_split) {
   typedef typename T::V V;
   constexpr int kRow = NP * DP * 2;             // bytes of an image row
   constexpr int KS = DP / 16, DT = DP / 32, RT = NP == 2 || WT ? 1 : 2;   // sub-tiles of 32 stream rows worked on together
@@ -392,6 +400,33 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
     }
   }
   l += __shfl_xor(l, 32);
+  if (BWD && grad.table) {
+    if (!inside) return;
+    typedef typename std::conditional<NP == 2, float, typename T::E>::type E;
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    const bool none = !seen || add == -INFINITY;
+    const float share = grad.mean ? 1.f / (float)max(1, *grad.valid) : 1.f, k = grad.scale * share;
+    const int up = none ? 0 : (int)m;
+    E* dst = reinterpret_cast<E*>(grad.table) + own_row * grad.d;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c0 = 32 * t + 8 * g + 4 * half;
+        E4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (E)(none ? 0.f : ldexpf(o[t][4 * g + e], up) * k);
+        if (grad.vec) {
+          if (c0 < grad.d) *reinterpret_cast<E4*>(dst + c0) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c0 + e < grad.d) dst[c0 + e] = v[e];
+        }
+      }
+    if (half == 0 && grad.bias) grad.bias[own_row] = none ? 0.f : ldexpf(l, up) * share;
+    return;
+  }
   const int64_t at = (int64_t)split * own.rows_pad + own_row;
   if (half == 0) {
     part.m[at] = seen ? m : -INFINITY;
@@ -931,7 +966,7 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
   int64_t at = 0;
   auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };
   const int64_t row = (int64_t)y.np * y.dp * 2;
-  const int64_t part = std::max((int64_t)y.fs * y.npad, grad ? (int64_t)y.bs * y.cpad : 0);
+  const int64_t part = std::max((int64_t)y.fs * y.npad, grad && y.bs > 1 ? (int64_t)y.bs * y.cpad : 0);
   y.u_img = take(y.npad * row);
   y.u_inv = take(y.npad * 4);
   y.u_h = take(y.npad * 4);
@@ -950,8 +985,11 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
   return y;
 }
 
-// Up to kFewRows rows: see xent_few_forward_kernel.
-constexpr int kFewRows = 4, kFewSplits = 256;
+// Up to four rows take the kernels of a few rows: one row of 17,000 x 100 fp32 24 us (47 through images and the matrix pipe), four 35 (48),
+// of 1M x 128 330 and 403 (574); in 16 bits, where the table is half the bytes and the matrix pipe needs a third of the products, four
+// rows only of a smaller table: 35 (38) at 17,000, but 471 (323) at 1M.
+constexpr int kFewRows = 4;
+inline bool few_rows(int64_t n, int64_t c, int32_t dtype) { return n == 1 || (n <= kFewRows && (dtype == NNCF_F32 || c < 131072)); }
 
 template <class T, int NP, int DP>
 int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
@@ -981,9 +1019,9 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
     const dim3 grid((unsigned)y.fs, (unsigned)(y.npad / kOwn));
     ProfScope ps("xent_stream_kernel", st);
     if (grad)
-      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, true>), grid, dim3(256), 0, st, u, v, part, scale2, stages, per);
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, true>), grid, dim3(256), 0, st, u, v, part, Grad{}, scale2, stages, per);
     else
-      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, false>), grid, dim3(256), 0, st, u, v, part, scale2, stages, per);
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, false>), grid, dim3(256), 0, st, u, v, part, Grad{}, scale2, stages, per);
   }
   const bool scalar = x->reduction != NNCF_NONE;
   const int mean = x->reduction == NNCF_MEAN;
@@ -1004,13 +1042,20 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
     if (scalar) hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, st, to);
   } else {
     const int stages = (int)(up(x->n, kTile) / kTile), per = (stages + y.bs - 1) / y.bs;
+    // d_table alone needs no joining where the users are not split: 0.5 GB less to write and to read at 1M items of 128
+    const Grad direct = y.bs == 1 ? Grad{x->d_table, x->d_bias, valid, x->scale, x->dim, mean, vec(x->d_table, x->dim)} : Grad{};
     const dim3 grid((unsigned)y.bs, (unsigned)(y.cpad / kOwn));
     {
       ProfScope ps("xent_stream_kernel", st);
       if (x->weight)
-        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, true, true>), grid, dim3(256), 0, st, v, u, part, scale2, stages, per);
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, true, true>), grid, dim3(256), 0, st, v, u, part, direct, scale2, stages, per);
       else
-        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, false, true>), grid, dim3(256), 0, st, v, u, part, scale2, stages, per);
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, false, true>), grid, dim3(256), 0, st, v, u, part, direct, scale2, stages, per);
+    }
+    if (y.bs == 1) {
+      if (scalar) hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, st, to);
+      NNCF_HIP_CHECK(hipGetLastError());
+      return NNCF_OK;
     }
     ProfScope ps("xent_table_kernel", st);
     constexpr int kRows = 256 / (DP / 4);
@@ -1026,7 +1071,7 @@ struct FewLayout {
 };
 FewLayout few_layout(int64_t n, int64_t c, bool grad) {
   FewLayout y{};
-  y.per = up((c + kFewSplits - 1) / kFewSplits, 64);
+  y.per = up(c / (c < 131072 ? 256 : 512) + 1, 64);     // more workgroups where there is work for them; their results are joined in turn
   y.splits = (int)((c + y.per - 1) / y.per);
   int64_t at = 0;
   auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };
@@ -1100,7 +1145,7 @@ int check_shape(int64_t n, int64_t c, int32_t dim, int32_t dtype) {
 
 extern "C" int64_t nncf_softmax_xent_ws_bytes(int64_t n, int64_t c, int32_t dim, int32_t dtype, int32_t with_grad) {
   if (nncf::check_shape(n, c, dim, dtype) != NNCF_OK) return -1;
-  if (n <= nncf::kFewRows) return nncf::few_layout(n, c, with_grad != 0).bytes;
+  if (nncf::few_rows(n, c, dtype)) return nncf::few_layout(n, c, with_grad != 0).bytes;
   return nncf::layout(n, c, dim, dtype, with_grad != 0).bytes;
 }
 
@@ -1118,7 +1163,7 @@ extern "C" int nncf_softmax_xent(const nncf_xent* x, void* d_ws, int64_t ws_byte
   const uintptr_t es = x->dtype == NNCF_F32 ? 4 : 2;
   NNCF_REQUIRE((uintptr_t)x->rows % es == 0 && (uintptr_t)x->table % es == 0 && (uintptr_t)x->d_rows % es == 0 &&
                (uintptr_t)x->d_table % es == 0, "a tensor is not aligned to its elements");
-  const bool few = x->n <= kFewRows;
+  const bool few = few_rows(x->n, x->c, x->dtype);
   const Layout y = few ? Layout{} : layout(x->n, x->c, x->dim, x->dtype, x->d_rows != nullptr);
   const int64_t need = few ? few_layout(x->n, x->c, x->d_rows != nullptr).bytes : y.bytes;
   NNCF_REQUIRE(ws_bytes >= need, "workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
