@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(256, 2) int8_scores_wide_kernel(Scores a, int6
 }
 
 // ---- up to 32 rows: the table is read once, straight into the operands -------------------------------------------------------------
-// A wave takes 32 items at a time, four times (16 reads of 1 KB in flight for rows of 128 codes), against all rows, which it holds.
+// A wave takes 32 items at a time, twice (8 reads of 1 KB in flight for rows of 128 codes), against all rows, which it holds.
 // FUSED: the rows come as floating point values, and every workgroup codes them for itself (m k <= kFused values) instead of waiting
 // for a launch that does it once.
 constexpr int kFused = 4096;
@@ -406,6 +406,7 @@ struct FloatRows {
   int vec;
 };
 
+constexpr int kItems = 2;   // blocks of 32 items of a wave
 template <class E, class X, bool FUSED>
 __global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRows f) {
   __shared__ __attribute__((aligned(16))) int8_t s_q[FUSED ? kFused : 16];
@@ -414,11 +415,11 @@ __global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRow
   const int8_t* qx = a.qx;
   const float* sx = a.sx;
   // the table's first 128 codes are asked for before anything else
-  const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * 128;
-  const int8_t* t[4];
-  i32x4 ahead[4][4];
+  const int64_t first = ((int64_t)blockIdx.x * 4 + wave) * (32 * kItems);
+  const int8_t* t[kItems];
+  i32x4 ahead[kItems][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < kItems; ++j) {
     t[j] = a.qt + min(first + 32 * j + col, a.c - 1) * a.pitch + half * 16;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -456,26 +457,26 @@ __global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRow
   }
   const int8_t* x = qx + min((int64_t)col, a.m - 1) * a.pitch + half * 16;
   if (first >= a.c) return;
-  i32x16 acc[4];
+  i32x16 acc[kItems];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = 0;
+  for (int j = 0; j < kItems; ++j) acc[j] = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < 2 || a.pitch > 64) {
       const i32x4 xk = *reinterpret_cast<const i32x4*>(x + 32 * k);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xk, ahead[j][k], acc[j], 0, 0, 0);
+      for (int j = 0; j < kItems; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xk, ahead[j][k], acc[j], 0, 0, 0);
     }
   for (int64_t k0 = 128; k0 < a.pitch; k0 += 64) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const i32x4 xk = *reinterpret_cast<const i32x4*>(x + k0 + 32 * k);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xk, *reinterpret_cast<const i32x4*>(t[j] + k0 + 32 * k), acc[j], 0, 0, 0);
+      for (int j = 0; j < kItems; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xk, *reinterpret_cast<const i32x4*>(t[j] + k0 + 32 * k), acc[j], 0, 0, 0);
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < kItems; ++j) {
     const int64_t item = first + 32 * j + col;
     if (item >= a.c) continue;
     const float st = a.st[item], cb = a.cb ? a.cb[item] : 0.f;
@@ -506,7 +507,7 @@ int run_quantize(const void* x, int64_t stride, int64_t n, int64_t k, int normal
 template <class E, class X, bool FUSED>
 int run_few(const Scores& a, const FloatRows& f, hipStream_t st) {
   ProfScope ps("int8_scores_kernel", st);
-  hipLaunchKernelGGL((int8_scores_few_kernel<E, X, FUSED>), dim3((unsigned)((a.c + 511) / 512)), dim3(256), 0, st, a, f);
+  hipLaunchKernelGGL((int8_scores_few_kernel<E, X, FUSED>), dim3((unsigned)((a.c + 128 * kItems - 1) / (128 * kItems))), dim3(256), 0, st, a, f);
   NNCF_HIP_CHECK(hipGetLastError());
   return NNCF_OK;
 }
