@@ -163,12 +163,13 @@ __device__ __forceinline__ typename T::V read_cols(const char* lds, int plane, i
   return __builtin_bit_cast(typename T::V, c);
 }
 
-// The streaming kernel.  BWD: own rows are items.  WT: row weights of either sign.  MEAN: the O sums are wanted.
-template <class T, int NP, int DP, bool BWD, bool WT, bool MEAN>
+// The streaming kernel.  DU: the columns in use, rounded up (of rows DP wide in their image).  BWD: own rows are items.  WT: row weights of
+// either sign.  MEAN: the O sums are wanted.
+template <class T, int NP, int DP, int DU, bool BWD, bool WT, bool MEAN>
 __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str, Part part, Grad grad, float scale2, int stages, int stages_per_split) {
   typedef typename T::V V;
   constexpr int kRow = NP * DP * 2;             // bytes of an image row
-  constexpr int KS = DP / 16, DT = DP / 32, RT = NP == 2 || WT ? 1 : 2;   // sub-tiles of 32 stream rows worked on together
+  constexpr int KS = (DU + 15) / 16, DT = (DU + 31) / 32, RT = NP == 2 || WT ? 1 : 2;   // sub-tiles of 32 stream rows worked on together
   __shared__ Stage<NP, DP> s_a, s_b;            // two objects, so that a read of one does not wait for the filling of the other
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int split = blockIdx.x;
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
           for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
+              if (!(hit_rows >> (32 * r + 8 * g) & 0xff)) continue;
               const int at = 32 * (r0 + r) + 8 * g + 4 * half;
               const int4 t4 = *reinterpret_cast<const int4*>(s_tgt + at);
               const float4 k4 = *reinterpret_cast<const float4*>(s_kq + at);
@@ -280,11 +282,14 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
                 const bool is = tv[e] == own_id;
                 // 2^exponent is at or above the coefficient; one that is 0 asks for nothing
                 const float need = kv[e] == 0.f ? -INFINITY : (float)__builtin_amdgcn_frexp_expf(kv[e]) - m;
-                top = fmaxf(top, is ? need : x);
+                top = fmaxf(top, is ? need : -INFINITY);
                 x = is ? -INFINITY : x;
               }
-              __builtin_amdgcn_sched_barrier(0);   // the rare branch must not set the kernel's register count
             }
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, d[r][i]);
         }
       }
       if (__any(top > kRaise || (!seen && top > -INFINITY))) {
@@ -991,7 +996,7 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
 constexpr int kFewRows = 4;
 inline bool few_rows(int64_t n, int64_t c, int32_t dtype) { return n == 1 || (n <= kFewRows && (dtype == NNCF_F32 || c < 131072)); }
 
-template <class T, int NP, int DP>
+template <class T, int NP, int DP, int DU>
 int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
   typedef typename std::conditional<NP == 2, float, typename T::E>::type E;
   const bool grad = x->d_rows != nullptr;
@@ -1019,9 +1024,9 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
     const dim3 grid((unsigned)y.fs, (unsigned)(y.npad / kOwn));
     ProfScope ps("xent_stream_kernel", st);
     if (grad)
-      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, true>), grid, dim3(256), 0, st, u, v, part, Grad{}, scale2, stages, per);
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, DU, false, false, true>), grid, dim3(256), 0, st, u, v, part, Grad{}, scale2, stages, per);
     else
-      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, false, false, false>), grid, dim3(256), 0, st, u, v, part, Grad{}, scale2, stages, per);
+      hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, DU, false, false, false>), grid, dim3(256), 0, st, u, v, part, Grad{}, scale2, stages, per);
   }
   const bool scalar = x->reduction != NNCF_NONE;
   const int mean = x->reduction == NNCF_MEAN;
@@ -1048,9 +1053,9 @@ int run(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
     {
       ProfScope ps("xent_stream_kernel", st);
       if (x->weight)
-        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, true, true>), grid, dim3(256), 0, st, v, u, part, direct, scale2, stages, per);
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, DU, true, true, true>), grid, dim3(256), 0, st, v, u, part, direct, scale2, stages, per);
       else
-        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, true, false, true>), grid, dim3(256), 0, st, v, u, part, direct, scale2, stages, per);
+        hipLaunchKernelGGL((xent_stream_kernel<T, NP, DP, DU, true, false, true>), grid, dim3(256), 0, st, v, u, part, direct, scale2, stages, per);
     }
     if (y.bs == 1) {
       if (scalar) hipLaunchKernelGGL(xent_loss_kernel, dim3(1), dim3(256), 0, st, to);
@@ -1132,6 +1137,15 @@ int run_few_rows(const nncf_xent* x, char* ws, hipStream_t st) {
   return run_few<E, 4>(x, ws, st);
 }
 
+// Products over the columns in use: at 96 of 128 a quarter of them less.
+template <class T, int NP>
+int run_width(const nncf_xent* x, const Layout& y, char* ws, hipStream_t st) {
+  if (x->dim <= 64) return run<T, NP, 64, 64>(x, y, ws, st);
+  if (x->dim <= 96) return run<T, NP, 128, 96>(x, y, ws, st);
+  if (x->dim <= 112) return run<T, NP, 128, 112>(x, y, ws, st);
+  return run<T, NP, 128, 128>(x, y, ws, st);
+}
+
 int check_shape(int64_t n, int64_t c, int32_t dim, int32_t dtype) {
   NNCF_REQUIRE(n > 0 && n <= (int64_t)kOwn * 65535, "n = %lld rows out of range (1..%lld)", (long long)n, (long long)kOwn * 65535);
   // own tiles of a launch are its grid's second dimension
@@ -1175,8 +1189,7 @@ extern "C" int nncf_softmax_xent(const nncf_xent* x, void* d_ws, int64_t ws_byte
     if (x->dtype == NNCF_F16) return run_few_rows<_Float16>(x, ws, st);
     return run_few_rows<__bf16>(x, ws, st);
   }
-  const bool wide = y.dp == 128;
-  if (x->dtype == NNCF_F32) return wide ? run<F16, 2, 128>(x, y, ws, st) : run<F16, 2, 64>(x, y, ws, st);
-  if (x->dtype == NNCF_F16) return wide ? run<F16, 1, 128>(x, y, ws, st) : run<F16, 1, 64>(x, y, ws, st);
-  return wide ? run<BF16, 1, 128>(x, y, ws, st) : run<BF16, 1, 64>(x, y, ws, st);
+  if (x->dtype == NNCF_F32) return run_width<F16, 2>(x, y, ws, st);
+  if (x->dtype == NNCF_F16) return run_width<F16, 1>(x, y, ws, st);
+  return run_width<BF16, 1>(x, y, ws, st);
 }

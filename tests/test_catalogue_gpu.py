@@ -103,7 +103,7 @@ def check(r, want, dtype, d, reduction, n, c):
 
 SHAPES = [(1, 1, 1), (1, 2, 3), (2, 63, 50), (3, 64, 64), (33, 65, 65), (31, 129, 100), (64, 1000, 128), (127, 517, 99), (128, 128, 4), (129, 2050, 127),
           (300, 77, 36), (5, 20011, 100), (1025, 300, 128), (513, 4099, 50),
-          (4, 4100, 128), (2, 300, 33), (6, 131073, 48), (70, 66003, 101)]
+          (4, 4100, 128), (2, 300, 33), (6, 131073, 48), (70, 66003, 101), (200, 3000, 96), (200, 3000, 112), (40, 500, 65), (150, 700, 97), (150, 700, 113)]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -193,6 +193,24 @@ def test_xent_rows_of_any_magnitude():
     small = f[:, 0].cpu() <= 1
     tol = 1e-4 * want["terms"]["table"][small] + 1e-30
     assert ((r.d_table.double().cpu() - want["d_table"])[small].abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,f", [(F16, 2.0 ** -18), (BF16, 2.0 ** -120), (F16, 2.0 ** 9), (F32, 2.0 ** -60)])
+@pytest.mark.parametrize("n", [3, 60])
+def test_xent_at_the_ends_of_a_type(n, dtype, f):
+    """Tables of f16's subnormal values, or near its largest; of bfloat16's and fp32's small ones: the scale brings the logits back."""
+    rows, table, target = make(n, 400, 40, F32, seed=2)
+    table = (table * f).to(dtype)
+    rows = rows.to(dtype)
+    scale = 10.0 / f if dtype != BF16 else 2.0 ** 100
+    r = catalogue.softmax_xent(rows, table, target, scale=scale, reduction="none")
+    want = oracle(rows, table, target, scale=scale, reduction="none")
+    assert want["zmax"] > 1 or dtype == BF16      # they are
+    fine = dtype == F32 or f > 1        # gradients of the other tables leave the type: held to the fp32 results alone
+    if fine:
+        check(r, want, dtype, 40, "none", n, 400)
+    else:
+        check(r._replace(d_rows=None), want, dtype, 40, "none", n, 400)
 
 
 def test_xent_strides_and_alignment():
@@ -311,7 +329,8 @@ def test_scores(m, c, k, dtype):
 
 
 @pytest.mark.parametrize("m,c,k,pad,off", [(1000, 8001, 100, 0, 0), (4100, 2000, 50, 0, 0), (2050, 4100, 128, 4, 4), (2000, 3999, 64, 30, 13),
-                                           (3000, 2244, 20, 0, 0), (300, 30000, 100, 0, 0), (3000, 2200, 300, 0, 0)])
+                                           (3000, 2244, 20, 0, 0), (300, 30000, 100, 0, 0), (3000, 2200, 300, 0, 0),
+                                           (4200, 4301, 300, 0, 0), (4100, 4356, 200, 4, 0)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_scores_of_many_rows(m, c, k, pad, off, dtype):
     """Launches of many workgroups: rows that start anywhere in a line, in rows of a wider matrix, whose other columns stay."""
@@ -336,6 +355,15 @@ def test_scores_write_only_their_columns(m):
     got = catalogue.int8_scores(x, catalogue.quantize_rows(t), out=out)
     assert got is out and torch.equal(out, catalogue.int8_scores(x, catalogue.quantize_rows(t)))
     assert (wide[:, :5] == 7).all() and (wide[:, 50:] == 7).all() and (wide[m] == 7).all()
+
+
+def test_scores_of_rows_that_codes_cannot_hold():
+    t = catalogue.quantize_rows(torch.randn(1000, 40, device=DEV))
+    for m in (3, 40):       # coded in the launch, and before it
+        x = torch.randn(m, 40, device=DEV)
+        x[1, 7] = math.nan
+        s = catalogue.int8_scores(x, t)
+        assert torch.isnan(s[1]).all() and torch.isfinite(s[0]).all() and torch.isfinite(s[2:]).all()
 
 
 def test_scores_of_no_rows():
