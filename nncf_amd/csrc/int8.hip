@@ -58,6 +58,7 @@ __device__ __forceinline__ uint64_t codes8(const float* x, Coder c) {
   return r;
 }
 
+// Bound by its bytes: 1M x 128 fp32 134 us, 644 MB at 4.8 TB/s (a copy of 1 GiB: 5.2); back to fp32 121 us, 5.3 TB/s.
 // One row per LR lanes, 8 columns a lane and step.  Rows of one step (LR = 8, 16) stay in registers between the two uses of a
 // value; longer ones are read twice, the second time from a cache.
 template <class E, int LR, bool ONE>
@@ -136,8 +137,8 @@ struct Scores {
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
 // (32 WM) x (32 WC) outputs per wave, RW x 2 waves; KB codes of every row a stage, two stages in turn, filled from global memory without a
 // register (1 KB per wave and instruction).  Chunks of 16 bytes are placed so that the 32 rows of an operand read meet every bank alike.
-// 128 codes a stage are whole lines: in halves, the tile of 128 x 256 took 165 us at 2,000 x 16,384 x 4,096, whatever lay ahead (two
-// stages or three) -- 22 bytes a cycle and CU, as halves of lines.
+// 128 codes a stage are whole lines: 2,000 x 16,384 x 4,096 took 165 us in halves of lines with tiles of 128 x 256, whether one stage lay
+// ahead or two, and takes 131-145 in whole ones with 256 x 256: 1.9-2.0 POP/s; the pipe was busy in 44% of its cycles before.
 typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 
@@ -395,6 +396,8 @@ __global__ void __launch_bounds__(256, 2) int8_scores_wide_kernel(Scores a, int6
 }
 
 // ---- up to 32 rows: the table is read once, straight into the operands -------------------------------------------------------------
+// Bound by the table's bytes: 1M x 128 codes 26 us, 5.1 TB/s where the last-level cache holds them, 33 from memory; with four blocks of 32
+// items a wave instead of two it was 35 (half the waves in flight).
 // A wave takes 32 items at a time, twice (8 reads of 1 KB in flight for rows of 128 codes), against all rows, which it holds.
 // FUSED: the rows come as floating point values, and every workgroup codes them for itself (m k <= kFused values) instead of waiting
 // for a launch that does it once.
