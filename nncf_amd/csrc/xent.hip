@@ -17,7 +17,7 @@
 // largest value into [2^13, 2^14): hi + lo then hold 22 bits of every value within 2^16 of the row's largest and an absolute 2^-38 of
 // it below; three products (hi hi, hi lo, lo hi) leave about 6e-8 of sum |a b|, as an fp32 sum does.  A coefficient 2^(y - M) is rounded to
 // two planes for fp32 tables, to the tables' own type for 16-bit ones (the targets', which carry the largest terms, to two of either).  No range of values is excluded
-// (the scale of a row of values below 2^-87 stops at 2^100).  The reference exponents M are whole numbers, so every rescaling is exact.
+// (the scale stops at 2^77: a row whose largest value is below 2^-80 is held in fewer bits).  The reference exponents M are whole numbers, so every rescaling is exact.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
     if (!inside) return;
     typedef typename std::conditional<NP == 2, float, typename T::E>::type E;
     typedef E E4 __attribute__((ext_vector_type(4)));
-    const bool none = !seen || add == -INFINITY;
+    const bool none = (!seen && l == l) || add == -INFINITY;   // a column of nothing but NaN stays that
     const float share = grad.mean ? 1.f / (float)max(1, *grad.valid) : 1.f, k = grad.scale * share;
     const int up = none ? 0 : (int)m;
     E* dst = reinterpret_cast<E*>(grad.table) + own_row * grad.d;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
   }
   const int64_t at = (int64_t)split * own.rows_pad + own_row;
   if (half == 0) {
-    part.m[at] = seen ? m : -INFINITY;
+    part.m[at] = seen ? m : -INFINITY;   // (a column of nothing but NaN too: its l says so)
     part.l[at] = l;
   }
   if (MEAN) {
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, 
 #pragma unroll
     for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     int b = 0;
-    if (top > 0.f && top < INFINITY) b = min(100, 14 - __builtin_amdgcn_frexp_expf(top));
+    if (top > 0.f && top < INFINITY) b = min(77, 14 - __builtin_amdgcn_frexp_expf(top));   // 2^15 2^77 and 2^23 rows stay below 2^127 in l
     inv = ldexpf(1.f, -b);
     shift = (float)b;
     f16x8 hi, lo;
@@ -597,11 +597,11 @@ __global__ void __launch_bounds__(256) xent_rows_kernel(RowsOut a, Part part) {
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   float l = 0.f, o0 = 0.f, o1 = 0.f;
   const bool some = top > -INFINITY;
-  if (has && some) {
+  if (has) {
     for (int k = lane; k < a.splits; k += 64) {
       const int64_t at = (int64_t)k * a.rows_pad + row;
-      const float mk = part.m[at];
-      if (mk > -INFINITY) l += part.l[at] * __builtin_amdgcn_exp2f(mk - top);
+      const float mk = part.m[at], lk = part.l[at];
+      if (mk > -INFINITY || lk != lk) l += mk > -INFINITY ? lk * __builtin_amdgcn_exp2f(mk - top) : lk;
     }
     l = wave_sum(l);
     if (MEAN) {
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(256) xent_rows_kernel(RowsOut a, Part part) {
     if (lane + 64 < a.d) { u1 = (float)u[lane + 64]; v1 = (float)v[lane + 64]; }
   }
   const float zt = out ? -INFINITY : fmaf(a.scale, wave_sum(fmaf(u1, v1, u0 * v0)), beta);
-  const float rest = some && !(l == 0.f) ? (top + log2f(l)) * kLn2 : -INFINITY;   // log sum over the other items
+  const float rest = l != l ? l : some && !(l == 0.f) ? (top + log2f(l)) * kLn2 : -INFINITY;   // log sum over the other items
   const float apart = rest - zt;
   float each, q, lse;
   if (out) {
@@ -915,12 +915,13 @@ __global__ void __launch_bounds__(256) xent_table_kernel(TableOut a, Part part) 
   for (int k = 0; k < a.splits; ++k) top = fmaxf(top, part.m[(int64_t)k * a.rows_pad + row]);
   float l = 0.f;
   float4 o = zero4();
-  if (top > -INFINITY && !out) {
+  if (!out) {
+    if (!(top > -INFINITY)) top = 0.f;       // nothing, or nothing but NaN
 #pragma unroll 4
     for (int k = 0; k < a.splits; ++k) {
       const int64_t at = (int64_t)k * a.rows_pad + row;
       const float mk = part.m[at], f = mk > -INFINITY ? __builtin_amdgcn_exp2f(mk - top) : 0.f;
-      l = fmaf(part.l[at], f, l);
+      l = fmaf(part.l[at], f, l);            // NaN * 0 is NaN: a split of nothing but NaN is not lost
       o = fma4(f, *reinterpret_cast<const float4*>(part.o + at * DP + 4 * q), o);
     }
     const float share = a.mean ? 1.f / (float)max(1, *a.valid) : 1.f;

@@ -161,6 +161,52 @@ def test_xent_rows_that_take_no_part():
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [2, 5, 200])
+def test_xent_values_that_are_no_numbers_are_not_lost(n, dtype):
+    rows, table, target = make(n, 700, 40, dtype)
+    for bad in (math.nan, math.inf):
+        item = table.clone()
+        item[699, 3] = bad                      # an item of the catalogue: every row's logits
+        r = catalogue.softmax_xent(rows, item, target.clamp(max=600))
+        if math.isnan(bad):
+            assert torch.isnan(r.loss) and torch.isnan(r.d_rows).all() and torch.isnan(r.d_table).all()
+        else:       # a row with a negative value there has the logit -inf, and only 0 * inf in its gradient
+            assert torch.isnan(r.loss) == bool((rows[:, 3] >= 0).any() or dtype == F32 or n > 4) or not torch.isfinite(r.loss)
+            assert torch.isnan(r.d_rows[:, 3]).all()
+        one = rows.clone()
+        one[1] = bad                            # a row: its loss, and every item's gradient
+        r = catalogue.softmax_xent(one, table, target, reduction="none")
+        assert torch.isnan(r.loss[1]) and torch.isnan(r.d_rows[1]).all() and torch.isnan(r.d_table).all()
+        assert torch.isfinite(r.loss[0]) and torch.isfinite(r.d_rows[0]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_xent_a_whole_part_of_nan_is_not_lost(dtype):
+    """NaN in every item (user) that one workgroup streams, and in no other."""
+    rows, table, target = make(300, 9000, 40, dtype)
+    item = table.clone()
+    item[4096:4096 + 512] = math.nan
+    r = catalogue.softmax_xent(rows, item, target.clamp(max=4000), reduction="none")
+    assert torch.isnan(r.loss).all() and torch.isnan(r.d_rows).all() and torch.isnan(r.d_table).all()
+    assert torch.isnan(catalogue.softmax_xent(rows[:3], item, target[:3].clamp(max=4000), reduction="none").loss).all()
+    user = rows.clone()
+    user[64:192] = math.nan
+    for sl in (slice(0, 9000), slice(0, 400)):
+        r = catalogue.softmax_xent(user, table[sl], target.clamp(max=399), reduction="none")
+        assert torch.isnan(r.loss[64:192]).all() and torch.isfinite(r.loss[:64]).all() and torch.isnan(r.d_table).all()
+
+
+def test_xent_of_tiny_rows():
+    """A table of 2^-79: full precision; the sums of its scales stay finite over many items."""
+    rows, table, target = make(40, 5000, 32, F32, seed=8)
+    table = table * 2.0 ** -76
+    kw = dict(scale=10.0 * 2.0 ** 76, reduction="none")
+    r = catalogue.softmax_xent(rows, table, target, **kw)
+    want = oracle(rows, table, target, **kw)
+    check(r._replace(d_rows=None), want, F32, 32, "none", 40, 5000)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_xent_confident_rows_keep_their_gradient(dtype):
     """p_t -> 1: the gradient is (1 - p_t) (mean of the others - v_t), down to 1 - p_t of 1e-13, where 1 - p_t by subtraction is 0."""
     c, d = 300, 64
