@@ -15,9 +15,10 @@
 //
 // Products of fp32 tables run on the f16 matrix pipe as two planes, x 2^b = hi + lo, with a power of two per ROW that brings its
 // largest value into [2^13, 2^14): hi + lo then hold 22 bits of every value within 2^16 of the row's largest and an absolute 2^-38 of
-// it below; three products (hi hi, hi lo, lo hi) leave about 6e-8 of sum |a b|, as an fp32 sum does.  A coefficient 2^(y - M) is rounded to
-// two planes for fp32 tables, to the tables' own type for 16-bit ones (the targets', which carry the largest terms, to two of either).  No range of values is excluded
-// (the scale stops at 2^77: a row whose largest value is below 2^-80 is held in fewer bits).  The reference exponents M are whole numbers, so every rescaling is exact.
+// it below; three products (hi hi, hi lo, lo hi) leave about 6e-8 of sum |a b|, as an fp32 sum does.  No range of values is excluded (the
+// scale stops at 2^77: a row whose largest value is below 2^-80 is held in fewer bits).  A coefficient 2^(y - M) is rounded to two planes
+// for fp32 tables and to the tables' own type for 16-bit ones; the targets', the largest terms of their sums, to two planes of either.
+// The reference exponents M are whole numbers, so every rescaling is exact.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
