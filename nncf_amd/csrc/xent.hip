@@ -943,19 +943,21 @@ __global__ void __launch_bounds__(256) xent_table_kernel(TableOut a, Part part) 
 // ---- host --------------------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Splits of the stream axis.  A launch runs in rounds of 512 workgroups (two on each of 256 CUs); a split costs its stages and about three
-// more (operands in, results out and joined).  In the backward pass a popular item's workgroup meets a target in every stage and takes
-// twice as long in it: it may become the launch's long pole.  Measured, backward: 1,000 x 50,021 f16 (391 own tiles, 16 stages) 97 us
-// with 1 split, 56 with 2, 76 with 8; 512 x 17,000 fp32 (133, 8) 56 / 37 / 31 / 33 / 39 us with 1 / 2 / 3 / 4 / 8; forward: 512 rows (4 own
-// tiles, 266 stages) 102 / 57 / 36 / 26 / 31 us with 8 / 16 / 32 / 64 / 256.
+// Splits of the stream axis.  A workgroup costs its stages and about three more (operands in, results out and joined); k of them on a CU
+// take 0.8 k times as long as one (two at a time overlap a little).  In the backward pass a popular item's workgroup meets a target in
+// every stage and takes up to three times as long in it: it may become the launch's long pole.  Measured, whole calls in us.  Forward, 512 x
+// 17,000 x 100 fp32 (4 own tiles, 266 stages): 106 / 84 / 74 / 77 / 85 / 90 with 16 / 32 / 54 / 89 / 133 / 256; 1,000 x 50,021 bf16 (8, 782):
+// 141 / 113 / 109 / 120 / 145 with 16 / 32 / 64 / 89 / 256.  Backward, the same two (133, 8): 90 / 80 / 74 / 78 / 80 / 89 with 1 / 2 / 3 / 4 /
+// 6 / 8; (391, 16): 110 / 105 / 110 / 113 / 142 with 1 / 2 / 3 / 4 / 8; 2,048 x 4,000 fp32 (32, 32): 236 / 153 / 109 / 92 / 87 / 102 with 1 / 2 / 4 /
+// 8 / 16 / 32.
 inline int splits_for(int64_t own_tiles, int64_t stages, bool backward) {
   int best = 1;
   int64_t least = INT64_MAX;
   for (int s = 1; s <= 256 && s <= stages; ++s) {
     const int64_t per = (stages + s - 1) / s;
     if ((stages + per - 1) / per != s) continue;    // the last split would be empty
-    const int64_t rounds = (own_tiles * s + 511) / 512;
-    const int64_t cost = std::max(rounds * (per + 3), backward ? 2 * per + 3 : 0);
+    const int64_t k = (own_tiles * s + 255) / 256;
+    const int64_t cost = std::max((k == 1 ? 10 : 8 * k) * (per + 3), backward ? 30 * per + 30 : 0);
     if (cost < least) {
       least = cost;
       best = s;
