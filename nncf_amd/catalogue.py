@@ -42,7 +42,7 @@ def _pitch(t):
 
 
 def _vector(t, name, n, dtype, device):
-    if t is None:
+    if t is None and name != "scale":
         return None
     if not isinstance(t, torch.Tensor) or t.device != device:
         raise TypeError("%s must be a tensor on %s" % (name, device))
@@ -118,12 +118,23 @@ def softmax_xent(rows, table, target, bias=None, weight=None, scale=1.0, reducti
 
 class Int8Rows(object):
     """Rows in 8 bits: `codes` int8 [n, pitch] (zeros behind the k-th column) and `scale` float32 [n]; row i stands for
-    codes[i, :k] * scale[i]."""
+    codes[i, :k] * scale[i].  Made by quantize_rows, or from codes and scales kept elsewhere (pitch = nncf_int8_pitch(k): 64 up to
+    k = 64, else the next multiple of 128)."""
 
     __slots__ = ("codes", "scale", "k")
 
     def __init__(self, codes, scale, k):
+        _matrix(codes, "codes", (torch.int8,))
+        if codes.shape[1] != _lib.lib().nncf_int8_pitch(k) or not codes.is_contiguous() or codes.data_ptr() % 16:
+            raise ValueError("codes of rows %d wide must be [n, %d], contiguous and 16-byte aligned" % (k, _lib.lib().nncf_int8_pitch(k)))
+        _vector(scale, "scale", codes.shape[0], torch.float32, codes.device)
         self.codes, self.scale, self.k = codes, scale, k
+
+    @classmethod
+    def _of(cls, codes, scale, k):
+        self = cls.__new__(cls)
+        self.codes, self.scale, self.k = codes, scale, k
+        return self
 
     def __len__(self):
         return self.codes.shape[0]
@@ -152,7 +163,7 @@ def quantize_rows(x, normalize=False):
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
     _call(x.device, L.nncf_quantize_rows, x.data_ptr(), _pitch(x), _DTYPES[x.dtype], n, k, int(bool(normalize)),
           codes.data_ptr(), scale.data_ptr())
-    return Int8Rows(codes, scale, k)
+    return Int8Rows._of(codes, scale, k)
 
 
 def int8_scores(rows, table, row_bias=None, col_bias=None, out=None, dtype=torch.float32):

@@ -403,6 +403,74 @@ def test_scores_write_only_their_columns(m):
     assert (wide[:, :5] == 7).all() and (wide[:, 50:] == 7).all() and (wide[m] == 7).all()
 
 
+def test_offsets_past_32_bits():
+    """A table of codes of 2.2 GB, scores of 9 GB, and a table whose rows lie 4.8 GB apart from first to last."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    c = 17_000_001
+    big = catalogue.Int8Rows(torch.randint(-127, 128, (c, 128), generator=g, device=DEV, dtype=torch.int8), torch.rand(c, generator=g, device=DEV), 128)
+    x = torch.randn(2, 128, generator=g, device=DEV)
+    s = catalogue.int8_scores(x, big)
+    last = catalogue.Int8Rows(big.codes[-1000:].clone(), big.scale[-1000:].clone(), 128)
+    assert torch.equal(s[:, -1000:], catalogue.int8_scores(x, last))
+    back = catalogue.Int8Rows(big.codes[-4:].clone(), big.scale[-4:].clone(), 128).dequantize()
+    assert torch.equal(big.dequantize(BF16)[-4:], back.to(BF16))
+    del big, s
+    m, c = 70_000, 33_001
+    x, t = (catalogue.quantize_rows(torch.randn(n, 30, generator=g, device=DEV)) for n in (m, c))
+    s = catalogue.int8_scores(x, t)
+    few = catalogue.Int8Rows(x.codes[-20:].clone(), x.scale[-20:].clone(), 30)
+    assert torch.equal(s[-20:], catalogue.int8_scores(few, t))
+    del s
+    c = 200_000
+    wide = torch.empty(c, 12_000, dtype=BF16, device=DEV)
+    table = wide[:, :32]
+    table.copy_(torch.randn(c, 32, generator=g, device=DEV) / 6)
+    target = torch.tensor([c - 1, 5, c - 3, 7, 9, c // 2], dtype=torch.int32, device=DEV)
+    rows = table[target.long()] * 2
+    r = catalogue.softmax_xent(rows, table, target, scale=10.0)
+    want = catalogue.softmax_xent(rows, table.contiguous(), target, scale=10.0)
+    for a, b in zip(r[:4], want[:4]):
+        assert torch.equal(a, b)
+
+
+def test_codes_kept_elsewhere():
+    x = torch.randn(9, 70, device=DEV)
+    r = catalogue.quantize_rows(x)
+    again = catalogue.Int8Rows(r.codes.clone(), r.scale.clone(), 70)
+    t = catalogue.quantize_rows(torch.randn(50, 70, device=DEV))
+    assert torch.equal(catalogue.int8_scores(again, t), catalogue.int8_scores(r, t))
+    for codes, scale, k in ((r.codes[:, :70], r.scale, 70), (r.codes, r.scale, 60), (r.codes, r.scale, 129), (r.codes, r.scale[:8], 70),
+                            (r.codes[:, :64], r.scale, 64), (r.codes, r.scale, 0)):
+        with pytest.raises(ValueError):
+            catalogue.Int8Rows(codes, scale, k)
+    for codes, scale, k in ((r.codes.float(), r.scale, 70), (r.codes, r.scale.double(), 70), (r.codes, None, 70), (r.codes.cpu(), r.scale, 70)):
+        with pytest.raises(TypeError):
+            catalogue.Int8Rows(codes, scale, k)
+
+
+def test_calls_that_are_refused():
+    rows, table, target = make(4, 50, 20, F32)
+    f = catalogue.softmax_xent
+    for call, error in ((lambda: f(rows, table.half(), target), TypeError), (lambda: f(rows, table[:, :10], target), ValueError),
+                        (lambda: f(rows, table, target.long()), TypeError), (lambda: f(rows, table, target[:3]), ValueError),
+                        (lambda: f(rows, table, None), TypeError), (lambda: f(rows, table, target, bias=torch.zeros(49, device=DEV)), ValueError),
+                        (lambda: f(rows, table, target, weight=torch.zeros(4)), TypeError), (lambda: f(rows, table, target, reduction="max"), ValueError),
+                        (lambda: f(rows, table, target, scale=math.inf), ValueError), (lambda: f(rows[:0], table, target[:0]), ValueError),
+                        (lambda: f(rows.t(), table, target), ValueError), (lambda: f(rows[:1].expand(4, 20), table, target), ValueError),
+                        (lambda: f(torch.zeros(4, 129, device=DEV), torch.zeros(50, 129, device=DEV), target), ValueError),
+                        (lambda: f(rows.double(), table.double(), target), TypeError), (lambda: f(rows[0], table, target), ValueError)):
+        with pytest.raises(error):
+            call()
+    t = catalogue.quantize_rows(table)
+    g = catalogue.int8_scores
+    for call, error in ((lambda: g(rows, table), TypeError), (lambda: g(rows[:, :19].contiguous(), t), ValueError),
+                        (lambda: g(rows, t, out=torch.empty(4, 49, device=DEV)), ValueError), (lambda: g(rows, t, dtype=torch.float64), TypeError),
+                        (lambda: g(rows, t, row_bias=torch.zeros(5, device=DEV)), ValueError), (lambda: g(rows, t, out=torch.empty(4, 50)), TypeError),
+                        (lambda: g(rows.double(), t), TypeError), (lambda: t.dequantize(torch.int8), TypeError)):
+        with pytest.raises(error):
+            call()
+
+
 def test_scores_of_rows_that_codes_cannot_hold():
     t = catalogue.quantize_rows(torch.randn(1000, 40, device=DEV))
     for m in (3, 40):       # coded in the launch, and before it
