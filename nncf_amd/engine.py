@@ -282,21 +282,29 @@ class Engine(object):
             _lib.check(self._L.nncf_gather_rows(_ptr(table), self.dim_p, self.dim_p, _ptr(ids), ids.numel(), 0, _ptr(out), self._stream()))
         return out
 
-    def softmax_xent(self, uid, cid, weight=None, reduction="mean", grad=True):
+    def softmax_xent(self, uid, cid, weight=None, reduction="mean", grad=True, scale=None):
         """Softmax cross entropy of the links (uid, cid) over ALL items -- what the schemes' sampled and shared negatives stand in for --
-        with logits loss_gamma * <u, v> (+ the item's interaction bias), and its gradients: XentResult with d_rows [n, dim] per link,
-        d_table [items, dim] and d_bias.  Nothing is updated.  A negative cid takes its link out.  Rows are used as the tables hold them:
-        an engine that normalises them (emb_normalization) is refused, and so is one whose item table is a text tower's block of a batch."""
+        with logits scale * s, s = <u, v> + the item's interaction bias: the score that predict_scores ranks by, as log-loss scales it
+        (a user's bias adds the same to all logits of its link).  scale: loss_gamma unless given; a max-margin engine's loss_gamma is a
+        margin, so there it has to be given.  Returns XentResult with d_rows [n, dim] per link, d_table [items, dim] and d_bias, the
+        gradients of the tables and the bias as this engine holds them.  Nothing is updated.  A negative cid takes its link out.  Rows are
+        used as the tables hold them: an engine that normalises them (emb_normalization) is refused, and so is one whose item table is a
+        text tower's block of a batch."""
         if self.cfg.normalize_user or self.cfg.normalize_item:
             raise ValueError("softmax_xent takes rows as they are; this engine normalises them")
         if getattr(self, "_export", None) is not None:
             raise ValueError("the item table of this engine is a batch's block of tower outputs, not the catalogue")
+        if scale is None:
+            if self.cfg.loss == _lib.LOSS_CODES["max-margin"]:
+                raise ValueError("loss_gamma of a max-margin engine is a margin, no scale of its scores: give scale")
+            scale = self.cfg.loss_gamma
         uid, cid = self.ids(uid), self.ids(cid)
         if uid.numel() != cid.numel():
             raise ValueError("%d users, %d items" % (uid.numel(), cid.numel()))
-        bias = self.bias["cb"] if self.bias is not None else None      # a user's bias adds the same to all of its logits
-        return catalogue.softmax_xent(self._rows(self.U, uid)[:, :self.dim], self.V[:, :self.dim], cid, bias=bias, weight=weight,
-                                      scale=self.cfg.loss_gamma, reduction=reduction, grad=grad)
+        cb = self.bias["cb"] if self.bias is not None else None
+        r = catalogue.softmax_xent(self._rows(self.U, uid)[:, :self.dim], self.V[:, :self.dim], cid, bias=None if cb is None else cb * scale,
+                                   weight=weight, scale=scale, reduction=reduction, grad=grad)
+        return r if r.d_bias is None else r._replace(d_bias=r.d_bias * scale)
 
     def quantize_items(self, cid):
         """The items `cid` in 8 bits (normalised where this engine normalises them), for predict_scores_int8."""
