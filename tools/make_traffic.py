@@ -78,7 +78,7 @@ def evaluator_entry(d, tag):
             "how": "rocprofv3 --kernel-trace --pmc FETCH_SIZE / --pmc WRITE_SIZE over tools/eval_bench.py, separate passes "
                    "(profiles/%s_eval_pmc_*.txt); bytes = (2*FETCH_SIZE + WRITE_SIZE) * 1024 per dispatch, mean over the train- and "
                    "the test-candidate launches; a whole@50 pass is one of each" % tag,
-            "round": int(tag.lstrip("r") or 0), "csrc_hash": source_hash()}
+            "csrc_hash": source_hash()}
 
 
 def main():
@@ -98,7 +98,6 @@ def main():
             "rocprof_avg_us": trace_avg_us(os.path.join(d, "%s_%s_kernel_trace.txt" % (tag, stem)), kernel),
             "how": "rocprofv3 --kernel-trace --pmc FETCH_SIZE / --pmc WRITE_SIZE, separate passes "
                    "(profiles/%s_%s_pmc_*.txt); bytes = (2*FETCH_SIZE + WRITE_SIZE) * 1024" % (tag, stem),
-            "round": int(tag.lstrip("r") or 0),
             "kernels": all_kernel_avgs(os.path.join(d, "%s_%s_kernel_trace.txt" % (tag, stem))),
             # bench.py trusts these durations only while the kernel sources are the ones that were profiled
             "csrc_hash": source_hash(),
