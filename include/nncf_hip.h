@@ -638,6 +638,8 @@ int nncf_int8_scores_rows(const void* d_x, int64_t x_stride, int32_t x_dtype, in
  *   d_req[n_ranks][cap] = the unique ids to request from each owner (ascending, -1 padded) and
  *   d_slot_of_pos[n] = request slot (owner * cap + k) holding the row of batch position i.
  * nncf_gather_rows: d_out[i][0..dim) = table row (d_ids[i] - id_offset) (zeros where d_ids[i] < 0).
+ * nncf_gather_rows_bias: the same for a table of `rows` rows and ids that nobody has checked, with a bias (NULL or [bias_rows]) of
+ *   each id: an id >= rows gives a row of NaN, one >= bias_rows a bias of NaN, a negative one zeros; nothing is read out of range.
  * nncf_scatter_apply: table[d_ids[i] - id_offset] -= lr * d_rows[i] for every i with d_ids[i] >= 0;
  *   rows of the same id are summed in list order first (deterministic, no atomics).  n <= 8192.
  * d_plan_ws: nncf_scatter_apply_ws_ints(n) int32 of 16-byte aligned scratch. */
@@ -645,6 +647,8 @@ int nncf_shard_route(const int32_t* d_cid, int32_t n, int32_t item_shard, int32_
                      int32_t* d_req, int32_t* d_slot_of_pos, int32_t* d_plan_ws, void* stream);
 int nncf_gather_rows(const float* d_table, int32_t row_stride, int32_t dim, const int32_t* d_ids, int64_t n,
                      int32_t id_offset, float* d_out, void* stream);
+int nncf_gather_rows_bias(const float* d_table, int64_t rows, int32_t row_stride, int32_t dim, const float* d_bias, int64_t bias_rows,
+                          const int32_t* d_ids, int64_t n, float* d_out, float* d_out_bias, void* stream);
 int nncf_scatter_apply(float* d_table, int32_t row_stride, int32_t dim, const int32_t* d_ids, int32_t n,
                        int32_t id_offset, const float* d_rows, float lr, int32_t* d_plan_ws, void* stream);
 int64_t nncf_scatter_apply_ws_ints(int32_t n);

@@ -131,6 +131,7 @@ def _declare(lib):
         "nncf_step_neg_shared_export": [vp, vp, vp, vp, vp, vp],
         "nncf_shard_route": [vp, i32, i32, i32, i32, vp, vp, vp, vp],
         "nncf_gather_rows": [vp, i32, i32, vp, i64, i32, vp, vp],
+        "nncf_gather_rows_bias": [vp, i64, i32, i32, vp, i64, vp, i64, vp, vp, vp],
         "nncf_shard_create": [vp, vp, i32, i32, i32, vp, i32, i32, i32, i32, i32, i32, ctypes.POINTER(vp)],
         "nncf_shard_destroy": [vp],
         "nncf_shard_counts": [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_int32)],

@@ -23,6 +23,21 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const float* __restric
   row_store(out, g, d, d4, q, id >= 0 ? row_load(table, id - id_offset, stride, d4, q) : row_zero());
 }
 
+// The same for ids that nobody has checked: one past the table (or the bias) reads nothing and gives NaN, a negative one zeros.  An id's
+// bias rides in the launch of its row.
+__global__ void __launch_bounds__(256) gather_rows_bias_kernel(const float* __restrict__ table, int64_t rows, int stride, int d,
+                                                               const float* __restrict__ bias, int64_t bias_rows,
+                                                               const int32_t* __restrict__ ids, int64_t n, float* __restrict__ out,
+                                                               float* __restrict__ out_bias) {
+  const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int q = threadIdx.x & 15, d4 = d >> 2;
+  if (g >= n) return;
+  const int id = ids[g];
+  const float4 none = make_float4(NAN, NAN, NAN, NAN);
+  row_store(out, g, d, d4, q, id < 0 ? row_zero() : id < rows ? row_load(table, id, stride, d4, q) : Row{none, none});
+  if (bias && q == 0) out_bias[g] = id < 0 ? 0.f : id < bias_rows ? bias[id] : NAN;
+}
+
 // Routing table of one sharded step (plan `pl` of the batch's item ids, ascending id order):
 // unique id with owner o = id / shard and rank k among o's ids goes to request slot o*cap + k.
 //   req[slot] = id (req pre-filled with -1), slot_of_pos[pos] = slot of the id at batch position pos.
@@ -154,6 +169,22 @@ extern "C" int nncf_gather_rows(const float* d_table, int32_t row_stride, int32_
     ProfScope _ps("gather_rows_kernel", as_stream(stream));
     hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, as_stream(stream), d_table,
                      row_stride, dim, d_ids, n, id_offset, d_out);
+  }
+  NNCF_HIP_CHECK(hipGetLastError());
+  return NNCF_OK;
+}
+
+extern "C" int nncf_gather_rows_bias(const float* d_table, int64_t rows, int32_t row_stride, int32_t dim, const float* d_bias,
+                                     int64_t bias_rows, const int32_t* d_ids, int64_t n, float* d_out, float* d_out_bias, void* stream) {
+  NNCF_REQUIRE(dim > 0 && dim % 4 == 0 && dim <= 128 && row_stride >= dim, "bad row shape");
+  NNCF_REQUIRE(rows >= 0 && bias_rows >= 0, "a table of %lld rows, %lld biases", (long long)rows, (long long)bias_rows);
+  NNCF_REQUIRE(n < (1LL << 28), "n = %lld rows out of range (below 2^28)", (long long)n);   // 16 lanes a row: fewer than 2^32 work items
+  if (n <= 0) return NNCF_OK;
+  NNCF_REQUIRE(d_table && d_ids && d_out && (!d_bias || d_out_bias), "NULL argument");
+  {
+    ProfScope _ps("gather_rows_kernel", as_stream(stream));
+    hipLaunchKernelGGL(gather_rows_bias_kernel, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, as_stream(stream), d_table, rows,
+                       row_stride, dim, d_bias, bias_rows, d_ids, n, d_out, d_out_bias);
   }
   NNCF_HIP_CHECK(hipGetLastError());
   return NNCF_OK;

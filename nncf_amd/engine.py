@@ -276,20 +276,24 @@ class Engine(object):
         return out
 
     # -- the catalogue head (nncf_amd/catalogue.py) on this engine's tables ----------------
-    def _rows(self, table, ids):
+    def _rows(self, table, ids, bias=None):
+        """Rows of `table` and, where there is a bias, its values: zeros for a negative id, NaN for one that the table does not hold."""
         out = torch.empty((ids.numel(), self.dim_p), dtype=torch.float32, device=self.device)
+        b = torch.empty(ids.numel(), dtype=torch.float32, device=self.device) if bias is not None else None
         with torch.cuda.device(self.device):
-            _lib.check(self._L.nncf_gather_rows(_ptr(table), self.dim_p, self.dim_p, _ptr(ids), ids.numel(), 0, _ptr(out), self._stream()))
-        return out
+            _lib.check(self._L.nncf_gather_rows_bias(_ptr(table), table.shape[0], self.dim_p, self.dim_p, _ptr(bias),
+                                                     bias.numel() if bias is not None else 0, _ptr(ids), ids.numel(), _ptr(out), _ptr(b),
+                                                     self._stream()))
+        return out, b
 
     def softmax_xent(self, uid, cid, weight=None, reduction="mean", grad=True, scale=None):
         """Softmax cross entropy of the links (uid, cid) over ALL items -- what the schemes' sampled and shared negatives stand in for --
         with logits scale * s, s = <u, v> + the item's interaction bias: the score that predict_scores ranks by, as log-loss scales it
         (a user's bias adds the same to all logits of its link).  scale: loss_gamma unless given; a max-margin engine's loss_gamma is a
         margin, so there it has to be given.  Returns XentResult with d_rows [n, dim] per link, d_table [items, dim] and d_bias, the
-        gradients of the tables and the bias as this engine holds them.  Nothing is updated.  A negative cid takes its link out.  Rows are
-        used as the tables hold them: an engine that normalises them (emb_normalization) is refused, and so is one whose item table is a
-        text tower's block of a batch."""
+        gradients of the tables and the bias as this engine holds them.  Nothing is updated.  A negative cid takes its link out.  A user or
+        an item that the tables do not hold makes the loss and the gradients NaN.  Rows are used as the tables hold them: an engine that
+        normalises them (emb_normalization) is refused, and so is one whose item table is a text tower's block of a batch."""
         if self.cfg.normalize_user or self.cfg.normalize_item:
             raise ValueError("softmax_xent takes rows as they are; this engine normalises them")
         if getattr(self, "_export", None) is not None:
@@ -302,23 +306,29 @@ class Engine(object):
         if uid.numel() != cid.numel():
             raise ValueError("%d users, %d items" % (uid.numel(), cid.numel()))
         cb = self.bias["cb"] if self.bias is not None else None
-        r = catalogue.softmax_xent(self._rows(self.U, uid)[:, :self.dim], self.V[:, :self.dim], cid, bias=None if cb is None else cb * scale,
+        r = catalogue.softmax_xent(self._rows(self.U, uid)[0][:, :self.dim], self.V[:, :self.dim], cid, bias=None if cb is None else cb * scale,
                                    weight=weight, scale=scale, reduction=reduction, grad=grad)
         return r if r.d_bias is None else r._replace(d_bias=r.d_bias * scale)
 
     def quantize_items(self, cid):
         """The items `cid` in 8 bits (normalised where this engine normalises them), for predict_scores_int8."""
-        return catalogue.quantize_rows(self._rows(self.V, self.ids(cid)), normalize=bool(self.cfg.normalize_item))
+        return catalogue.quantize_rows(self._rows(self.V, self.ids(cid))[0], normalize=bool(self.cfg.normalize_item))
 
     def predict_scores_int8(self, uid, cid, items=None, out=None):
-        """predict_scores from rows in 8 bits: users are quantised on the way in, items are quantize_items(cid) (made here if not given)."""
+        """predict_scores from rows in 8 bits: users are quantised on the way in, items are quantize_items(cid) (made here if not given).
+        A negative id stands for a row of zeros without a bias, an id that the tables do not hold for scores of NaN."""
         uid, cid = self.ids(uid), self.ids(cid)
-        items = self.quantize_items(cid) if items is None else items
-        users = self._rows(self.U, uid)
-        users = catalogue.quantize_rows(users, normalize=True) if self.cfg.normalize_user else users
         b = self.bias or {}
-        return catalogue.int8_scores(users, items, row_bias=b["ub"][uid.long()] if b.get("ub") is not None else None,
-                                     col_bias=b["cb"][cid.long()] if b.get("cb") is not None else None, out=out)
+        users, ub = self._rows(self.U, uid, b.get("ub"))
+        if items is None:
+            rows, cb = self._rows(self.V, cid, b.get("cb"))
+            items = catalogue.quantize_rows(rows, normalize=bool(self.cfg.normalize_item))
+        else:
+            if len(items) != cid.numel():
+                raise ValueError("%d items in 8 bits, %d ids" % (len(items), cid.numel()))
+            cb = self._rows(self.V, cid, b["cb"])[1] if b.get("cb") is not None else None
+        users = catalogue.quantize_rows(users, normalize=True) if self.cfg.normalize_user else users
+        return catalogue.int8_scores(users, items, row_bias=ub, col_bias=cb, out=out)
 
     def close(self):
         h, self._h = getattr(self, "_h", None), None

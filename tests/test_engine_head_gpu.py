@@ -72,3 +72,60 @@ def test_a_margin_is_no_scale():
     with pytest.raises(ValueError, match="margin"):
         e.softmax_xent([1, 2], [3, 4])
     assert torch.isfinite(e.softmax_xent([1, 2], [3, 4], scale=2.0).loss)
+
+
+@pytest.mark.parametrize("bias", [None, "both"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_ids_that_the_tables_do_not_hold(norm, bias):
+    """Past the tables: NaN, for that user or item alone.  Negative: a row of zeros without a bias.  Nothing is read out of range."""
+    e = engine(norm=norm, bias=bias)
+    top = 2 ** 31 - 1
+    uid, cid = np.array([3, 200, -1, 7, top, -2 ** 31]), np.array([0, 333, 5, -1, top, 332, -2 ** 31])
+    known_u, known_c = np.array([0, 3]), np.array([0, 2, 5])         # places of ids that are there
+    zero_u, zero_c = np.array([2, 5]), np.array([3, 6])
+    want = e.predict_scores_int8(uid[known_u], cid[known_c])
+    for items in (None, e.quantize_items(cid)):
+        s = e.predict_scores_int8(uid, cid, items=items)
+        assert torch.equal(s[known_u][:, known_c], want)
+        assert torch.isnan(s[[1, 4]]).all() and torch.isnan(s[:, [1, 4]]).all()
+        ub, cb = (torch.zeros(len(i), device="cuda") if bias is None else e.bias[k][torch.as_tensor(i, device="cuda")]
+                  for k, i in (("ub", uid[known_u]), ("cb", cid[known_c])))
+        assert torch.equal(s[zero_u][:, known_c], cb.expand(2, 3)) and torch.equal(s[known_u][:, zero_c], ub[:, None].expand(2, 2))
+        assert not s[zero_u][:, zero_c].any()
+
+
+def test_links_that_the_tables_do_not_hold():
+    e = engine(bias="both")
+    uid, cid = np.array([3, 200, 5, 2 ** 31 - 1]), np.array([1, -1, 7, -1])
+    r = e.softmax_xent(uid, cid, reduction="none")       # such a user in a link that takes no part
+    want = e.softmax_xent(uid[[0, 2]], cid[[0, 2]], reduction="none")
+    assert torch.equal(r.loss[[0, 2]], want.loss) and not r.loss[[1, 3]].any() and not r.d_rows[[1, 3]].any()
+    assert torch.isfinite(r.d_table).all()
+    for n in (3, 40):                                    # few rows, many rows
+        u, c = np.arange(n), np.arange(n)
+        u[1], c[2] = 200, 333
+        r = e.softmax_xent(u, c, reduction="none")
+        assert torch.isnan(r.loss[1:3]).all() and torch.isfinite(r.loss[0]) and torch.isfinite(r.loss[3:]).all()
+        assert torch.isnan(r.d_rows[1:3]).all() and torch.isfinite(r.d_rows[3:]).all() and torch.isnan(r.d_table).all()
+
+
+def test_items_in_8_bits_of_another_number_than_the_ids():
+    e = engine()
+    coded = e.quantize_items(np.arange(20))
+    with pytest.raises(ValueError, match="20 items"):
+        e.predict_scores_int8([1, 2], np.arange(19), items=coded)
+    with pytest.raises(ValueError, match="20 items"):
+        e.predict_scores_int8([1, 2], np.arange(333), items=coded)
+
+
+@pytest.mark.parametrize("d,n", [(50, 1), (100, 33), (128, 1000)])
+def test_gathered_rows_and_biases(d, n):
+    e = engine(d, bias="both")
+    ids = torch.randint(-3, 210, (n,), generator=torch.Generator().manual_seed(n)).int().cuda()
+    rows, b = e._rows(e.U, ids, e.bias["ub"])
+    there, past = (ids >= 0) & (ids < 200), ids >= 200
+    at = torch.where(there, ids, 0).long()
+    assert torch.equal(rows[there], e.U[at][there]) and torch.equal(b[there], e.bias["ub"][at][there])
+    assert torch.isnan(rows[past]).all() and torch.isnan(b[past]).all()
+    assert not rows[ids < 0].any() and not b[ids < 0].any()
+    assert e._rows(e.U, ids)[1] is None and e._rows(e.U, ids[:0], e.bias["ub"])[0].shape == (0, e.dim_p)
