@@ -868,7 +868,8 @@ __global__ void __launch_bounds__(256) xent_few_backward_kernel(Few a) {
       few_logits<N>(u, v[k], scale2, b2[k], y);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float w = out ? 0.f : j == t[i] ? -kq[i] : sg[i] * __builtin_amdgcn_exp2f(y[i] + h[i]);
+        if (out) continue;                    // left out: zeros whatever the rows hold (0 * NaN is none)
+        const float w = j == t[i] ? -kq[i] : sg[i] * __builtin_amdgcn_exp2f(y[i] + h[i]);
         sum += w;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = fmaf(w, u[i][e], x[e]);
