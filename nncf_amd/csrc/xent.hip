@@ -147,6 +147,13 @@ __device__ __forceinline__ void filled() {   // this wave's part has arrived, an
   __syncthreads();
 }
 
+// sum + kept += x, with what the addition rounds away in kept (two-sum: any signs and sizes)
+__device__ __forceinline__ void add_kept(float& sum, float& kept, float x) {
+  const float s = sum + x, b = s - sum;
+  kept += (sum - (s - b)) + (x - b);
+  sum = s;
+}
+
 template <class T, int NP, int DP>
 __device__ __forceinline__ typename T::V read_rows(const char* lds, int row, int plane, int chunk) {
   return *reinterpret_cast<const typename T::V*>(lds + lds_at<NP, DP>(row, plane, chunk));
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
   f32x16 o[MEAN ? DT : 1];
 #pragma unroll
   for (int d = 0; d < (MEAN ? DT : 1); ++d) o[d] = 0.f;
-  float m = 0.f, l = 0.f;
+  float m = 0.f, l = 0.f, lc = 0.f;             // the sum is l + lc
   bool seen = false;
 
   auto work = [&](const Stage<NP, DP>& st, int64_t row0) __attribute__((always_inline)) {
@@ -310,6 +317,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
         seen = seen || move;
         m += by;
         l *= f;
+        lc *= f;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -335,14 +343,20 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
             d[r][4 * g + 3] *= w4.w;
           }
       }
+      // The normaliser: a sub-tile's terms in four short sums, and those into a sum that keeps what its rounding loses.  One running fp32 sum
+      // of a million equal terms was off by up to 7e-4.
+      {
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          // 2^b = 1 / 2^-b, by its exponent
-          if (NP == 2) l = fmaf(d[r][i], __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, iv[r][i])), l);
-          else l += d[r][i];
-        }
+          for (int i = 0; i < 16; ++i) {
+            // 2^b = 1 / 2^-b, by its exponent
+            if (NP == 2) t[i & 3] = fmaf(d[r][i], __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, iv[r][i])), t[i & 3]);
+            else t[i & 3] += d[r][i];
+          }
+        add_kept(l, lc, (t[0] + t[1]) + (t[2] + t[3]));
+      }
       if (MEAN) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
@@ -370,6 +384,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
           for (int w = 0; w < 2 * RT; ++w) {
             if (!(hit_rows >> (16 * w) & 0xffff)) continue;
             V hi, lo;
+            float sum = 0.f;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const int at = 32 * r0 + 16 * w + 8 * g + 4 * half;
@@ -384,9 +399,10 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
                 const float v = tv[e] == own_id ? -ldexpf(kv[e], (int)-m) : 0.f;
                 hi[4 * g + e] = (typename T::E)v;
                 lo[4 * g + e] = (typename T::E)(v - (float)hi[4 * g + e]);
-                l += NP == 2 ? v * __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, ivv[e])) : v;
+                sum += NP == 2 ? v * __builtin_bit_cast(float, 0x7F000000 - __builtin_bit_cast(int, ivv[e])) : v;
               }
             }
+            add_kept(l, lc, sum);
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
               const V a = read_cols<T, NP, DP>(s_img, 0, 32 * r0 + 16 * w, t, lane);
@@ -414,6 +430,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
       filled();
     }
   }
+  l += lc;
   l += __shfl_xor(l, 32);
   if (BWD && grad.table) {
     if (!inside) return;
