@@ -33,6 +33,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
 constexpr int kOwn = 128;      // own rows of a workgroup: 4 waves x 32
 constexpr int kTile = 64;      // stream rows of a stage
+constexpr int kAside = 64;    // stages after which a workgroup's sums of rows are put aside
 constexpr float kTop = 10.f;   // a new reference puts the largest exponent of a row at <= 2^10 ...
 constexpr float kRaise = 15.f; // ... and is taken again once one passes 2^15 (f16 ends at 2^16)
 
@@ -416,6 +417,32 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
     }
   };
   const int t0 = split * stages_per_split, t1 = min(stages, t0 + stages_per_split);
+  // The O sums of kAside stages are one fp32 chain of the matrix pipe; those of a longer stream are added up in memory, beside their
+  // reference, by the lanes that hold them.  (Equal terms, 8,192 rows x 1M fp32, one chain a split: the mean item off by 3e-4.)
+  const int64_t aside0 = (int64_t)split * own.rows_pad + own0;      // of the wave; the lane's part is formed anew each time (asm: not kept)
+  auto lane_again = [&] {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto put_aside = [&](bool first) {
+    const int x = lane_again();
+    float* const to_m = part.m + aside0 + (x & 31);
+    float* const to_o = part.o + aside0 * DP + ((x & 31) * DP + 4 * (x >> 5));
+    const float f = first ? 0.f : __builtin_amdgcn_exp2f(*to_m - m);
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float4* p = reinterpret_cast<float4*>(to_o + 32 * t + 8 * g);
+        float4 v = make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
+        if (!first) v = fma4(f, *p, v);
+        *p = v;
+      }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = 0.f;
+    *to_m = seen ? m : -INFINITY;         // both halves of a column, the same value
+  };
   if (t0 < t1) {
     const Filler<NP, DP> filler(wave, lane);
     fill<NP, DP, BWD, WT>(s_a, filler, str, (int64_t)t0 * kTile, wave, lane);
@@ -428,6 +455,22 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
       if (tile + 2 < t1) fill<NP, DP, BWD, WT>(s_a, filler, str, (int64_t)(tile + 2) * kTile, wave, lane);
       work(s_b, (int64_t)(tile + 1) * kTile);
       filled();
+      if (MEAN && (tile + 2 - t0) % kAside == 0 && tile + 2 < t1) put_aside(tile + 2 - t0 == kAside);
+    }
+    if (MEAN && t1 - t0 > kAside) {
+      const int x = lane_again();
+      const float* const from_o = part.o + aside0 * DP + ((x & 31) * DP + 4 * (x >> 5));
+      const float f = __builtin_amdgcn_exp2f(part.m[aside0 + (x & 31)] - m);
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 v = *reinterpret_cast<const float4*>(from_o + 32 * t + 8 * g);
+          o[t][4 * g] = fmaf(f, v.x, o[t][4 * g]);
+          o[t][4 * g + 1] = fmaf(f, v.y, o[t][4 * g + 1]);
+          o[t][4 * g + 2] = fmaf(f, v.z, o[t][4 * g + 2]);
+          o[t][4 * g + 3] = fmaf(f, v.w, o[t][4 * g + 3]);
+        }
     }
   }
   l += lc;
@@ -1002,7 +1045,9 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
   int64_t at = 0;
   auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };
   const int64_t row = (int64_t)y.np * y.dp * 2;
-  const int64_t part = std::max((int64_t)y.fs * y.npad, grad && y.bs > 1 ? (int64_t)y.bs * y.cpad : 0);
+  // the backward pass needs room where it is split, and where it puts sums aside
+  const bool room = grad && (y.bs > 1 || up(n, kTile) / kTile > kAside);
+  const int64_t part = std::max((int64_t)y.fs * y.npad, room ? (int64_t)y.bs * y.cpad : 0);
   y.u_img = take(y.npad * row);
   y.u_inv = take(y.npad * 4);
   y.u_h = take(y.npad * 4);
@@ -1107,7 +1152,8 @@ struct FewLayout {
 };
 FewLayout few_layout(int64_t n, int64_t c, bool grad) {
   FewLayout y{};
-  y.per = up(c / (c < 131072 ? 256 : 512) + 1, 64);     // more workgroups where there is work for them; their results are joined in turn
+  // more workgroups where there is work for them; their results are joined in turn.  At most 4,096 items: 256 terms of a running sum.
+  y.per = std::min<int64_t>(up(c / (c < 131072 ? 256 : 512) + 1, 64), 4096);
   y.splits = (int)((c + y.per - 1) / y.per);
   int64_t at = 0;
   auto take = [&at](int64_t b) { const int64_t r = at; at += up(b, 256); return r; };

@@ -65,3 +65,77 @@ def test_the_bias_gradient_of_equal_terms(n, c, w, dtype):
     assert (r.d_bias[1:].double() / (k * n / c) - 1).abs().max().item() <= COEF + 30 * E
     # the target's: 1 - p_t of each user, to 4 roundings, and its sums
     assert abs(r.d_bias[0].item() / (k * n * (1 / c - 1)) - 1) <= LSE / c + 40 * E
+
+
+U = {t: torch.finfo(t).eps / 2 for t in (F32, F16, BF16)}
+# A sum of coefficient times value over many stream rows, relative to the sum of absolute terms.  At most 64 stages of 64 rows are one chain of
+# the matrix pipe: 3 products (two planes of either side) of 16 rows each, 768 accumulations, each rounding by E of a running sum that grows
+# evenly: 384 E.  Up to 64 such sums one after another and 256 splits in four shares, growing evenly too: 32 + 32.  Values and coefficients in
+# two planes: 4 + 4.  The division, the scales, the result: 8.  Coefficients of 16-bit tables are rounded to their type, all alike here: U.
+CHAIN = (384 + 32 + 32 + 8 + 8) * E
+
+
+def chain(dtype):
+    return CHAIN + (0 if dtype == F32 else 2 * U[dtype])        # (and the output's own rounding)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,c", [(4096, 1_000_000), (8192, 1_000_003), (130, 1_000_000), (20_000, 300_000), (4, 8_000_000)])
+def test_the_mean_item_of_equal_terms(n, c, dtype):
+    table, bias, r = long_rows(n, c, 16, dtype, 0.123, scale=2.0)
+    mean = table.double().sum(0) / c                   # the targets' rows are zeros: their weight 1 / c adds nothing
+    # 1 - p_t and the sum of the others' coefficients, whose exponents and reference are those of the rows' sum: 30 as the bias gradient's
+    assert ((r.d_rows.double() / (2 * mean) - 1).abs() <= chain(dtype) + 30 * E).all()
+
+
+def near(got, want, tol):
+    """Relative; a value past the type's largest, 65,504 for float16 (100,000 users' 0.7 sum up to 70,019), is that infinity."""
+    top = torch.finfo(got.dtype).max
+    past = want.abs() > top * (1 + tol)
+    got = got.double()
+    assert ((got / want - 1).abs() <= tol)[~past].all()
+    assert (got == torch.sign(want) * math.inf)[past].all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,c", [(8192, 40_000), (100_000, 40_000), (70_001, 300), (300_000, 35_000)])
+@pytest.mark.parametrize("w", [None, -0.7])
+def test_the_table_gradient_of_equal_terms(n, c, w, dtype):
+    weight = None if w is None else torch.full((n,), w, device="cuda")
+    k = 1.0 if w is None else weight[0].item()
+    rows, r = many_users(n, c, 16, dtype, weight)
+    want = k * rows.double().sum(0)
+    near(r.d_table[1:], (want / c).expand(c - 1, -1), chain(dtype) + COEF)
+    # the target's: all users, in windows of 16 rows with three products each, no other terms
+    near(r.d_table[0], want * (1 / c - 1), chain(dtype) + 40 * E)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,c", [(40, 3_000_000), (9000, 70_000)])
+def test_a_long_stream_whose_largest_terms_come_late(n, c, dtype):
+    """Logits that rise by 40 over the catalogue: sums put aside are brought to each new reference.  Against torch in 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    d = 24
+    table = (torch.randn(c, d, generator=g, device="cuda") / 8).to(dtype)
+    rows = torch.randn(n, d, generator=g, device="cuda").to(dtype)
+    bias = torch.linspace(-40, 0, c, device="cuda")
+    bias[: c // 2] = -math.inf                          # and many stages of nothing before them
+    target = (c - 1 - torch.arange(n, device="cuda") % 1000).int()
+    r = catalogue.softmax_xent(rows, table, target, bias=bias, reduction="none")
+    at = slice(c // 2, c)
+    v, b = table[at].double(), bias[at].double()
+    lse = torch.empty(n, dtype=torch.float64, device="cuda")
+    mean, dots = torch.empty(n, d, dtype=torch.float64, device="cuda"), 0.0
+    sure = torch.empty_like(mean)
+    for i in range(0, n, 100):
+        z = rows[i:i + 100].double() @ v.t() + b
+        lse[i:i + 100] = torch.logsumexp(z, 1)
+        p = torch.exp(z - lse[i:i + 100, None])
+        mean[i:i + 100], sure[i:i + 100] = p @ v, p @ v.abs()
+    dots = (rows.double().abs().sum(1).max() * v.abs().max()).item()
+    # a logit: planes and the fp32 sum of d products, and the exponent's additions of values up to 64 + 40
+    z_err = ((3 * 2.0 ** -22 if dtype == F32 else 0) + (d + 2) * E) * dots + 4 * E * 104
+    assert (r.lse.double() - lse).abs().max().item() <= 2 * z_err + LSE
+    vt = table[target.long()].double()
+    tol = (chain(dtype) + 2 * z_err + LSE) * (sure + vt.abs()) + U[dtype] * (mean - vt).abs()
+    assert ((r.d_rows.double() - (mean - vt)).abs() <= tol).all()
