@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 #include "devutil.h"
@@ -417,31 +418,50 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
     }
   };
   const int t0 = split * stages_per_split, t1 = min(stages, t0 + stages_per_split);
-  // The O sums of kAside stages are one fp32 chain of the matrix pipe; those of a longer stream are added up in memory, beside their
-  // reference, by the lanes that hold them.  (Equal terms, 8,192 rows x 1M fp32, one chain a split: the mean item off by 3e-4.)
-  const int64_t aside0 = (int64_t)split * own.rows_pad + own0;      // of the wave; the lane's part is formed anew each time (asm: not kept)
-  auto lane_again = [&] {
+  // The sums of kAside stages are put aside in memory, beside their reference, by the lanes that hold them, and begun anew.  Running on, O was
+  // one fp32 chain of the matrix pipe (equal terms, 8,192 rows x 1M fp32: the mean item off by 3e-4), and coefficients of 16 bits that are
+  // 2^35 below the largest of the whole stream, not of kAside stages, were lost.
+  const int64_t aside0 = (int64_t)split * own.rows_pad + own0;      // of the wave
+  auto lane_again = [&] {                                           // for addresses that are formed anew each time: not kept in the loop
     int x = lane;
     asm volatile("" : "+v"(x));
     return x;
   };
-  auto put_aside = [&](bool first) {
+  auto join_aside = [&](bool first, auto&& take) __attribute__((always_inline)) {
     const int x = lane_again();
-    float* const to_m = part.m + aside0 + (x & 31);
-    float* const to_o = part.o + aside0 * DP + ((x & 31) * DP + 4 * (x >> 5));
-    const float f = first ? 0.f : __builtin_amdgcn_exp2f(*to_m - m);
+    float* const at_m = part.m + aside0 + (x & 31);                 // both halves of a column, the same values
+    float* const at_l = part.l + aside0 + (x & 31);
+    float* const at_o = part.o + aside0 * DP + ((x & 31) * DP + 4 * (x >> 5));
+    const float before = first ? -INFINITY : *at_m, top = seen ? fmaxf(before, m) : before;
+    // nothing seen on either side: zeros, or NaN, which stays
+    const float fb = top > -INFINITY ? __builtin_amdgcn_exp2f(before - top) : 1.f, f = seen ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+    l += lc;
+    l += __shfl_xor(l, 32);
+    l *= f;
+    if (!first) l = fmaf(fb, *at_l, l);
+    if (MEAN) {
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float4* p = reinterpret_cast<float4*>(to_o + 32 * t + 8 * g);
-        float4 v = make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
-        if (!first) v = fma4(f, *p, v);
-        *p = v;
-      }
+        for (int g = 0; g < 4; ++g) {
+          float4* p = reinterpret_cast<float4*>(at_o + 32 * t + 8 * g);
+          float4 v = make_float4(o[t][4 * g] * f, o[t][4 * g + 1] * f, o[t][4 * g + 2] * f, o[t][4 * g + 3] * f);
+          if (!first) v = fma4(fb, *p, v);
+          take(t, g, v, p);
+          if (g & 1) __builtin_amdgcn_sched_barrier(0);             // two reads in flight: more would take registers from the loop
+        }
+    }
+    m = top;
+    return std::pair<float*, float*>(at_m, at_l);
+  };
+  auto put_aside = [&](bool first) {
+    const auto at = join_aside(first, [](int, int, float4 v, float4* p) { *p = v; });
+    *at.first = m;
+    *at.second = l;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = 0.f;
-    *to_m = seen ? m : -INFINITY;         // both halves of a column, the same value
+    for (int t = 0; t < (MEAN ? DT : 1); ++t) o[t] = 0.f;
+    m = l = lc = 0.f;
+    seen = false;
   };
   if (t0 < t1) {
     const Filler<NP, DP> filler(wave, lane);
@@ -455,34 +475,31 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
       if (tile + 2 < t1) fill<NP, DP, BWD, WT>(s_a, filler, str, (int64_t)(tile + 2) * kTile, wave, lane);
       work(s_b, (int64_t)(tile + 1) * kTile);
       filled();
-      if (MEAN && (tile + 2 - t0) % kAside == 0 && tile + 2 < t1) put_aside(tile + 2 - t0 == kAside);
-    }
-    if (MEAN && t1 - t0 > kAside) {
-      const int x = lane_again();
-      const float* const from_o = part.o + aside0 * DP + ((x & 31) * DP + 4 * (x >> 5));
-      const float f = __builtin_amdgcn_exp2f(part.m[aside0 + (x & 31)] - m);
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 v = *reinterpret_cast<const float4*>(from_o + 32 * t + 8 * g);
-          o[t][4 * g] = fmaf(f, v.x, o[t][4 * g]);
-          o[t][4 * g + 1] = fmaf(f, v.y, o[t][4 * g + 1]);
-          o[t][4 * g + 2] = fmaf(f, v.z, o[t][4 * g + 2]);
-          o[t][4 * g + 3] = fmaf(f, v.w, o[t][4 * g + 3]);
-        }
+      if ((tile + 2 - t0) % kAside == 0 && tile + 2 < t1) put_aside(tile + 2 - t0 == kAside);
     }
   }
-  l += lc;
-  l += __shfl_xor(l, 32);
+  if (t1 - t0 > kAside) {
+    join_aside(false, [&](int t, int g, float4 v, float4*) {
+      o[t][4 * g] = v.x;
+      o[t][4 * g + 1] = v.y;
+      o[t][4 * g + 2] = v.z;
+      o[t][4 * g + 3] = v.w;
+    });
+    seen = m > -INFINITY;
+    if (!seen) m = 0.f;
+  } else {
+    l += lc;
+    l += __shfl_xor(l, 32);
+  }
+  const int64_t row = own0 + (lane_again() & 31);
   if (BWD && grad.table) {
-    if (!inside) return;
+    if (row >= own.rows) return;
     typedef typename std::conditional<NP == 2, float, typename T::E>::type E;
     typedef E E4 __attribute__((ext_vector_type(4)));
     const bool none = (!seen && l == l) || add == -INFINITY;   // a column of nothing but NaN stays that
     const float share = grad.mean ? 1.f / (float)max(1, *grad.valid) : 1.f, k = grad.scale * share;
     const int up = none ? 0 : (int)m;
-    E* dst = reinterpret_cast<E*>(grad.table) + own_row * grad.d;
+    E* dst = reinterpret_cast<E*>(grad.table) + row * grad.d;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -499,10 +516,10 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
             if (c0 + e < grad.d) dst[c0 + e] = v[e];
         }
       }
-    if (half == 0 && grad.bias) grad.bias[own_row] = none ? 0.f : ldexpf(l, up) * share;
+    if (half == 0 && grad.bias) grad.bias[row] = none ? 0.f : ldexpf(l, up) * share;
     return;
   }
-  const int64_t at = (int64_t)split * own.rows_pad + own_row;
+  const int64_t at = (int64_t)split * own.rows_pad + row;
   if (half == 0) {
     part.m[at] = seen ? m : -INFINITY;   // (a column of nothing but NaN too: its l says so)
     part.l[at] = l;
@@ -589,8 +606,10 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, 
     for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
 #pragma unroll
     for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    int b = 0;
-    if (top > 0.f && top < INFINITY) b = min(77, 14 - __builtin_amdgcn_frexp_expf(top));   // 2^15 2^77 and 2^23 rows stay below 2^127 in l
+    // 2^15 2^77 and 2^23 rows stay below 2^127 in l.  A row of zeros goes as one of 2^-27: it adds nothing to O, and its coefficient should not set
+    // the reference of those that do.
+    int b = top > 0.f ? 0 : 40;
+    if (top > 0.f && top < INFINITY) b = min(77, 14 - __builtin_amdgcn_frexp_expf(top));
     inv = ldexpf(1.f, -b);
     shift = (float)b;
     f16x8 hi, lo;

@@ -139,3 +139,32 @@ def test_a_long_stream_whose_largest_terms_come_late(n, c, dtype):
     vt = table[target.long()].double()
     tol = (chain(dtype) + 2 * z_err + LSE) * (sure + vt.abs()) + U[dtype] * (mean - vt).abs()
     assert ((r.d_rows.double() - (mean - vt)).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n,c", [(32_768, 262_144), (130, 131_072), (4, 300_000)])
+@pytest.mark.parametrize("down", [30.6, 35.1, 38.6])
+def test_a_tail_far_below_the_largest_term(n, c, down):
+    """One item and 2^-down of it in each of the others: a coefficient is held to 2^-25 of a largest one of at least 2^9, and what that loses
+    is no more than the 4,096 terms of kAside stages, 2^-22 of the largest in all."""
+    d = 8
+    table = torch.zeros(c, d, device="cuda")
+    table[:, 0] = 1.0
+    table[5, 0] = table[c - 1, 0] = 0.0
+    bias = torch.full((c,), -down * math.log(2), device="cuda")
+    bias[5] = 0.0
+    target = torch.full((n,), c - 1, device="cuda").int()
+    r = catalogue.softmax_xent(torch.zeros(n, d, device="cuda"), table, target, bias=bias, reduction="none")
+    tail = math.exp(bias[0].item())
+    want = (c - 2) * tail / (1 + (c - 1) * tail)
+    assert (r.d_rows[:, 0].double() - want).abs().max().item() <= 2.0 ** -22 + (CHAIN + COEF) * want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_loss_alone_is_the_same(dtype):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = (torch.randn(600_000, 24, generator=g, device="cuda") / 5).to(dtype)
+    rows = torch.randn(5000, 24, generator=g, device="cuda").to(dtype)
+    target = torch.randint(600_000, (5000,), generator=g, device="cuda").int()
+    a = catalogue.softmax_xent(rows, table, target, scale=3.0, reduction="none")
+    b = catalogue.softmax_xent(rows, table, target, scale=3.0, reduction="none", grad=False)
+    assert torch.equal(a.loss, b.loss) and torch.equal(a.lse, b.lse)
