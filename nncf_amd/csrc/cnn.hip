@@ -1177,12 +1177,14 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdThreads == 512 ? 4 : 1) cnn_c
     __syncthreads();
     cnn_stamp(a, 1, 3);
     float xb[KPW][kCnnCWB / 4];   // the words' rows of the strip: requested now, used by (b) right behind the barrier
+    int kh = kq, xh = x;          // this pass's own: the 24 + 6 sums of them with constants are formed here, not kept over the passes (spills)
+    asm volatile("" : "+v"(kh), "+v"(xh));
 #pragma unroll
     for (int ks = 0; ks < KPW; ++ks) {
       const int kt = wave + NW * ks, kcol = kt * 16 + x;
 #pragma unroll
       for (int st = 0; st < kCnnCWB / 4; ++st) {
-        const int cl = 4 * st + kq;
+        const int cl = 4 * st + kh;
         xb[ks][st] = (kt < nKw && cl < ncl && kcol < wd) ? a.W[(int64_t)ix.cw[c0 + cl] * wd + kcol] : 0.f;
       }
     }
@@ -1273,7 +1275,7 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdThreads == 512 ? 4 : 1) cnn_c
             }
 #pragma unroll
             for (int mt = 0; mt < 3; ++mt) {
-              const int cl = 16 * (mh + mt) + x;
+              const int cl = 16 * (mh + mt) + xh;
               if (mh + mt < nmt && cl < ncl && k0 < wd) {
                 float4* dst = reinterpret_cast<float4*>(dxw + ((int64_t)s * L + ix.cj[c0 + cl]) * wd + k0);
                 float4 v = make_float4(acc[mt][0], acc[mt][1], acc[mt][2], acc[mt][3]);

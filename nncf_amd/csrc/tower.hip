@@ -779,6 +779,7 @@ __global__ void __launch_bounds__(512, (CNN || MAXP) ? 6 : 8) tower_word_kernel(
   __shared__ int sList[8 * kListCap];
   __shared__ float2 sAccW[8 * kWordsPerWG * 64];  // [wave][word][lane]
   __shared__ int sHit[kWordsPerWG];
+  __shared__ int sEnd[PM ? kWordsPerWG : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int G = PM ? a.pm_nwg : (a.n_words + kWordsPerWG - 1) / kWordsPerWG;
   // CNN tower: the first workgroups of the grid sum the dWk partials and update the conv weights, conv
@@ -865,27 +866,29 @@ __global__ void __launch_bounds__(512, (CNN || MAXP) ? 6 : 8) tower_word_kernel(
   const float2* dh2 = reinterpret_cast<const float2*>(cnn ? a.cnn.dXw : a.dh);
   __syncthreads();
   unsigned long long hit_bits[2] = {0ull, 0ull};   // (pass, word) pairs in which this lane found a cell: up to 16 passes
-  int pbeg[kWordsPerWG], pend[kWordsPerWG];
+  int pbeg[kWordsPerWG];
   int rounds = 0;
   if (PM) {
 #pragma unroll
     for (int j = 0; j < kWordsPerWG; ++j) {
       const int4 u = a.pm_units[(int64_t)bid * kWordsPerWG + j];
       const int w = u.x;
-      pbeg[j] = pend[j] = 0;
+      pbeg[j] = 0;
+      int pend = 0;
       if (w >= 0 && !(a.skip_words & 4)) {
         bool skip = a.train && word_scale(a, w) == 0.f;
         if (a.hot_bits) skip = skip || ((a.hot_bits[w >> 5] >> (w & 31)) & 1u);
         if (!skip) {
           pbeg[j] = u.y;
-          pend[j] = u.z;
+          pend = u.z;
         }
       }
       // workgroup-uniform (the unit table and the dropout hash of a word are): scalar registers -- as sixteen VECTOR registers
       // they were what the 64-register budget of four workgroups per CU lacked (4 spilled to scratch: round 5 audit)
       pbeg[j] = __builtin_amdgcn_readfirstlane(pbeg[j]);
-      pend[j] = __builtin_amdgcn_readfirstlane(pend[j]);
-      rounds = max(rounds, (pend[j] - pbeg[j] + 511) >> 9);
+      pend = __builtin_amdgcn_readfirstlane(pend);
+      rounds = max(rounds, (pend - pbeg[j] + 511) >> 9);
+      sEnd[j] = pend;                 // (every wave the same, each reads its own: sixteen scalars over the walk were eight too many)
     }
   }
   for (int base = 0; base < (PM ? 0 : n); base += 512 * NB) {
@@ -1057,7 +1060,7 @@ __global__ void __launch_bounds__(512, (CNN || MAXP) ? 6 : 8) tower_word_kernel(
 #pragma unroll
       for (int j = 0; j < kWordsPerWG; ++j) {
         const int e = pbeg[j] + 512 * r + 64 * wave + lane;
-        pk[j] = e < pend[j] ? a.post_item[e] : 0xFFFFFFFFu;
+        pk[j] = e < sEnd[j] ? a.post_item[e] : 0xFFFFFFFFu;
       }
 #pragma unroll
       for (int j = 0; j < kWordsPerWG; ++j) sv[j] = pk[j] != 0xFFFFFFFFu ? a.slot_of[pk[j] & 0xFFFFFFu] : make_int2(0, 0);
