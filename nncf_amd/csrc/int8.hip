@@ -491,18 +491,42 @@ __global__ void __launch_bounds__(256) int8_scores_few_kernel(Scores a, FloatRow
   }
 }
 
+// A launch holds fewer than 2^32 work items: this many workgroups of 256 at most, longer calls in pieces.
+constexpr int64_t kMostBlocks = 1LL << 23;
+
+template <class E, int LR, bool ONE>
+void launch_quantize(const E* x, int64_t stride, int64_t n, int64_t k, int vec, int normalize, int8_t* q, float* scale, hipStream_t st) {
+  constexpr int kRows = 256 / LR;      // of a workgroup
+  const int64_t pitch = pitch_of(k);
+  for (int64_t at = 0; at < n; at += kMostBlocks * kRows) {
+    const int64_t rows = std::min(n - at, kMostBlocks * kRows);
+    hipLaunchKernelGGL((quantize_rows_kernel<E, LR, ONE>), dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(256), 0, st, x + at * stride, stride,
+                       rows, k, vec, normalize, q + at * pitch, scale + at);
+  }
+}
+
 template <class E>
 int run_quantize(const void* x, int64_t stride, int64_t n, int64_t k, int normalize, int8_t* q, float* scale, hipStream_t st) {
   const E* p = reinterpret_cast<const E*>(x);
   const int vec = (uintptr_t)x % (4 * sizeof(E)) == 0 && stride % 4 == 0;
   const int64_t pitch = pitch_of(k);
   ProfScope ps("quantize_rows_kernel", st);
-  if (pitch == 64)
-    hipLaunchKernelGGL((quantize_rows_kernel<E, 8, true>), dim3((unsigned)((n + 31) / 32)), dim3(256), 0, st, p, stride, n, k, vec, normalize, q, scale);
-  else if (pitch == 128)
-    hipLaunchKernelGGL((quantize_rows_kernel<E, 16, true>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, p, stride, n, k, vec, normalize, q, scale);
-  else
-    hipLaunchKernelGGL((quantize_rows_kernel<E, 64, false>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, p, stride, n, k, vec, normalize, q, scale);
+  if (pitch == 64) launch_quantize<E, 8, true>(p, stride, n, k, vec, normalize, q, scale, st);
+  else if (pitch == 128) launch_quantize<E, 16, true>(p, stride, n, k, vec, normalize, q, scale, st);
+  else launch_quantize<E, 64, false>(p, stride, n, k, vec, normalize, q, scale, st);
+  NNCF_HIP_CHECK(hipGetLastError());
+  return NNCF_OK;
+}
+
+template <class E>
+int run_dequantize(const int8_t* q, const float* scale, int64_t n, int64_t k, void* out, hipStream_t st) {
+  const int64_t groups = (k + 7) / 8, most = kMostBlocks * 256 / groups;     // rows of a piece: at least 131,072
+  ProfScope ps("dequantize_rows_kernel", st);
+  for (int64_t at = 0; at < n; at += most) {
+    const int64_t rows = std::min(n - at, most);
+    hipLaunchKernelGGL((dequantize_rows_kernel<E>), dim3((unsigned)((rows * groups + 255) / 256)), dim3(256), 0, st, q + at * pitch_of(k), scale + at,
+                       rows, k, groups, reinterpret_cast<E*>(out) + at * k);
+  }
   NNCF_HIP_CHECK(hipGetLastError());
   return NNCF_OK;
 }
@@ -518,7 +542,7 @@ int run_few(const Scores& a, const FloatRows& f, hipStream_t st) {
 template <class E, int WM, int WC, int RW, int KB>
 int run_many(const Scores& a, hipStream_t st) {
   const int64_t mt = (a.m + 32 * WM * RW - 1) / (32 * WM * RW), ct = (a.c + 64 * WC - 1) / (64 * WC);
-  NNCF_REQUIRE(mt * ct < (1LL << 30), "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
+  NNCF_REQUIRE(mt * ct <= kMostBlocks - 8, "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);      // (of up to 512 threads)
   const int vec = a.c % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(E)) == 0;
   const dim3 grid((unsigned)((mt * ct + 7) / 8 * 8));
   ProfScope ps("int8_scores_kernel", st);
@@ -528,11 +552,23 @@ int run_many(const Scores& a, hipStream_t st) {
 }
 
 template <class E>
-int run_scores(const Scores& a, hipStream_t st) {
+int run_scores(Scores a, hipStream_t st) {
+  constexpr int64_t kRows = 1LL << 22;      // of a piece: few columns of very many rows are more workgroups than a launch takes
+  while (a.m > kRows) {
+    Scores piece = a;
+    piece.m = kRows;
+    const int rc = run_scores<E>(piece, st);
+    if (rc) return rc;
+    a.qx += kRows * a.pitch;
+    a.sx += kRows;
+    if (a.rb) a.rb += kRows;
+    a.out = reinterpret_cast<E*>(a.out) + kRows * a.out_stride;
+    a.m -= kRows;
+  }
   if (a.m <= 32) return run_few<E, float, false>(a, FloatRows{}, st);
   const int64_t wide_c = (a.c + kWideStep - 1) / kWideStep, wide = (a.m + kWideRows - 1) / kWideRows * wide_c;
   if (a.pitch <= 128 && wide >= 256) {
-    NNCF_REQUIRE(wide < (1LL << 30), "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
+    NNCF_REQUIRE(wide <= kMostBlocks - 8, "%lld x %lld scores in one call", (long long)a.m, (long long)a.c);
     const bool vec = a.c % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % (4 * sizeof(E)) == 0;
     const dim3 grid((unsigned)((wide + 7) / 8 * 8));
     ProfScope ps("int8_scores_kernel", st);
@@ -591,21 +627,10 @@ extern "C" int nncf_dequantize_rows(const int8_t* d_q, const float* d_scale, int
   if (n == 0) return NNCF_OK;
   NNCF_REQUIRE(d_q && d_scale && d_out, "NULL argument");
   NNCF_REQUIRE(((uintptr_t)d_q & 15) == 0 && ((uintptr_t)d_out & 15) == 0, "codes and output must be 16-byte aligned");
-  const int64_t groups = (k + 7) / 8, blocks = (n * groups + 255) / 256;
-  NNCF_REQUIRE(blocks < (1LL << 31), "%lld x %d values in one call", (long long)n, k);
   hipStream_t st = as_stream(stream);
-  {
-    ProfScope ps("dequantize_rows_kernel", st);
-    const dim3 grid((unsigned)blocks);
-    if (dtype == NNCF_F32)
-      hipLaunchKernelGGL((dequantize_rows_kernel<float>), grid, dim3(256), 0, st, d_q, d_scale, n, (int64_t)k, groups, (float*)d_out);
-    else if (dtype == NNCF_F16)
-      hipLaunchKernelGGL((dequantize_rows_kernel<_Float16>), grid, dim3(256), 0, st, d_q, d_scale, n, (int64_t)k, groups, (_Float16*)d_out);
-    else
-      hipLaunchKernelGGL((dequantize_rows_kernel<__bf16>), grid, dim3(256), 0, st, d_q, d_scale, n, (int64_t)k, groups, (__bf16*)d_out);
-  }
-  NNCF_HIP_CHECK(hipGetLastError());
-  return NNCF_OK;
+  if (dtype == NNCF_F32) return run_dequantize<float>(d_q, d_scale, n, k, d_out, st);
+  if (dtype == NNCF_F16) return run_dequantize<_Float16>(d_q, d_scale, n, k, d_out, st);
+  return run_dequantize<__bf16>(d_q, d_scale, n, k, d_out, st);
 }
 
 extern "C" int nncf_int8_scores(const int8_t* d_qx, const float* d_sx, int64_t m, const int8_t* d_qt, const float* d_st, int64_t c, int32_t k,

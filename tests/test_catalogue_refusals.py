@@ -95,3 +95,10 @@ def test_host_tensors_are_refused():
                  lambda: catalogue.softmax_xent(x.numpy(), x, t)):
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("m,c,k", [(1 << 22, 1 << 31, 100), (1 << 22, 300_000, 60), (1 << 22, 1 << 18, 300)])
+def test_more_scores_than_a_launch_holds_are_refused(m, c, k):
+    """2^32 work items: refused as an argument, not as a launch that fails (such a matrix has a terabyte)."""
+    with pytest.raises(ValueError, match="in one call"):
+        _lib.check(_lib.lib().nncf_int8_scores(P, P, m, P, P, c, k, None, None, P, c, 0, None))
