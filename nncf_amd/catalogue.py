@@ -117,9 +117,9 @@ def softmax_xent(rows, table, target, bias=None, weight=None, scale=1.0, reducti
 
 
 class Int8Rows(object):
-    """Rows in 8 bits: `codes` int8 [n, pitch] (zeros behind the k-th column) and `scale` float32 [n]; row i stands for
+    """Rows in 8 bits: `codes` int8 [n, pitch] (-127 .. 127, zeros behind the k-th column) and `scale` float32 [n]; row i stands for
     codes[i, :k] * scale[i].  Made by quantize_rows, or from codes and scales kept elsewhere (pitch = nncf_int8_pitch(k): 64 up to
-    k = 64, else the next multiple of 128)."""
+    k = 64, else the next multiple of 128): those are read once here, which waits for the device and is refused while a graph is captured."""
 
     __slots__ = ("codes", "scale", "k")
 
@@ -128,6 +128,13 @@ class Int8Rows(object):
         if codes.shape[1] != _lib.lib().nncf_int8_pitch(k) or not codes.is_contiguous() or codes.data_ptr() % 16:
             raise ValueError("codes of rows %d wide must be [n, %d], contiguous and 16-byte aligned" % (k, _lib.lib().nncf_int8_pitch(k)))
         _vector(scale, "scale", codes.shape[0], torch.float32, codes.device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("codes made elsewhere are read when they are taken over: do that before the capture")
+        # the products rely on both: sums of 127^2 k stay below 2^31, and columns behind the k-th are multiplied like the others
+        for i in range(0, codes.shape[0], 1 << 22):
+            part = codes[i:i + (1 << 22)]
+            if part[:, :k].amin() < -127 or part[:, k:].any():
+                raise ValueError("codes are -127 .. 127, and zeros behind the first %d columns" % k)
         self.codes, self.scale, self.k = codes, scale, k
 
     @classmethod
