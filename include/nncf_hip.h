@@ -581,14 +581,17 @@ typedef enum { NNCF_NONE = 0, NNCF_MEAN = 1, NNCF_SUM = 2 } nncf_reduction;
  *   reduction NNCF_SUM: loss[0] = sum of loss_i; NNCF_MEAN: that over the number of rows with a target (0 rows: loss 0);
  *   NNCF_NONE: loss[n].  d_rows[n][dim], d_table[c][dim], d_bias[c]: the gradients of loss[0] (NNCF_NONE: of the sum of loss_i,
  *   so that weight carries an upstream gradient).  The n x c values are never stored; sums are kept in 32 bits, nothing is added
- *   in a varying order.
+ *   in a varying order.  Equal terms of any number leave lse within 1.2e-5, the gradients within 5e-5 of themselves (beside the rounding of
+ *   16-bit types).  fp32 rows: meant for largest values of 2^-80 .. 2^90 in rows within 2^100 of each other (above 2^-27 beside 16
+ *   adjacent rows of zeros); a gradient may miss 2^-22 of its largest term in terms that are 2^-34 of it or less.
  * - rows, table, d_rows, d_table hold elements of `dtype`; strides in elements, any alignment of their own type (16-byte aligned
  *   rows of a multiple of 4 elements are read fastest); the gradients are contiguous.  dim <= 128 (any), as every row of this library.
  * - target_i < 0: the row takes no part (loss 0, lse 0, gradient 0, its values are not used).  target_i >= c: NaN loss and gradients.
  * - bias_j = -inf: item j is left out (its row is not used, its gradient is 0).  A row whose target is left out, or that has no item
  *   left, has loss +inf and no gradient.
- * - weight (NULL = 1): any finite value, 0 and negative ones too.  bias NULL = 0.
- * - d_rows and d_table: both or neither (loss only); d_bias NULL or with a bias.  1 <= n, c <= 128 * 65535.
+ * - weight (NULL = 1): any finite value, 0 and negative ones too.  A row whose values are not all finite reaches the gradients of the items
+ *   that are not left out, at weight 0 too: a negative target takes it out.  bias NULL = 0.
+ * - d_rows and d_table: both or neither (loss only; the same loss and lse); d_bias NULL or with a bias.  1 <= n, c <= 128 * 65535.
  * The workspace (256-byte aligned, nncf_softmax_xent_ws_bytes; -1 for a shape that is refused) holds nothing between calls; calls
  * that may run at the same time need one each. */
 typedef struct nncf_xent {
@@ -615,14 +618,15 @@ int nncf_softmax_xent(const nncf_xent* x, void* d_ws, int64_t ws_bytes, void* st
 /* Rows in 8 bits: code = rint(x * (127 / top)), scale = top / 127 with top = max |x| of the row, each operation in fp32.  d_q holds
  * rows of nncf_int8_pitch(k) bytes (64 up to k = 64, else the next multiple of 128; zeros behind the k-th), 16-byte aligned.  A row of
  * zeros has scale 0; a row with an infinity or NaN has zero codes and scale NaN.  normalize: the scale is that of the L2-normalised
- * row (x * rsqrt(max(sum x^2, 1e-12)), model_framework.py:62-63).  k <= 131072. */
+ * row (x * rsqrt(max(sum x^2, 1e-12)), model_framework.py:62-63).  k <= 131072, n <= 2^31 (in several launches where one does not hold it). */
 int64_t nncf_int8_pitch(int32_t k);
 int nncf_quantize_rows(const void* d_x, int64_t x_stride, int32_t dtype, int64_t n, int32_t k, int32_t normalize, int8_t* d_q,
                        float* d_scale, void* stream);
 /* d_out[n][k] = code * scale, 16-byte aligned. */
 int nncf_dequantize_rows(const int8_t* d_q, const float* d_scale, int64_t n, int32_t k, void* d_out, int32_t dtype, void* stream);
-/* d_out[i][j] = sx_i * st_j * sum_k qx_ik qt_jk + row_bias_i + col_bias_j (biases NULL or fp32), the integer sum exact; rows of
- * d_out are out_stride elements of `dtype` apart, columns beyond c are not written. */
+/* d_out[i][j] = sx_i * st_j * sum_k qx_ik qt_jk + row_bias_i + col_bias_j (biases NULL or fp32), the integer sum exact: codes are -127 .. 127
+ * and zeros behind the k-th, which is not checked here; rows of d_out are out_stride elements of `dtype` apart, columns beyond c are not
+ * written.  m, c <= 2^31; a matrix of more tiles than a launch holds (a terabyte) is refused. */
 int nncf_int8_scores(const int8_t* d_qx, const float* d_sx, int64_t m, const int8_t* d_qt, const float* d_st, int64_t c, int32_t k,
                      const float* d_row_bias, const float* d_col_bias, void* d_out, int64_t out_stride, int32_t dtype, void* stream);
 

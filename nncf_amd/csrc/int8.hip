@@ -3,7 +3,7 @@
 //   top = max |x|, code = rint(x (127 / top)), scale = top / 127          out_ij = scale_i scale_j sum_k code_ik code_jk + biases
 //
 // Codes lie in rows of nncf_int8_pitch(k) bytes, zeros behind the k-th: whole steps of the integer matrix instruction, 16-byte
-// aligned.  The integer sum is exact (k <= 131,072: 127^2 k < 2^31), so nothing depends on the order of a sum.
+// aligned.  The integer sum is exact (codes of -127 .. 127, k <= 131,072: 127^2 k < 2^31), so nothing depends on the order of a sum.
 #include <algorithm>
 #include <cmath>
 
@@ -138,7 +138,7 @@ struct Scores {
 // (32 WM) x (32 WC) outputs per wave, RW x 2 waves; KB codes of every row a stage, two stages in turn, filled from global memory without a
 // register (1 KB per wave and instruction).  Chunks of 16 bytes are placed so that the 32 rows of an operand read meet every bank alike.
 // 128 codes a stage are whole lines: 2,000 x 16,384 x 4,096 took 165 us in halves of lines with tiles of 128 x 256, whether one stage lay
-// ahead or two, and takes 131-145 in whole ones with 256 x 256: 1.9-2.0 POP/s; the pipe was busy in 44% of its cycles before.
+// ahead or two, and takes 147 (best of 40: 129) in whole ones with 256 x 256: 1.8-2.1 POP/s, the pipe busy in 57% of its cycles (44% before).
 typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 
@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(128 * RW, 2) int8_scores_kernel(Scores a, int6
 // The output is all there is to do: 4 bytes a value against 128 codes.  Its rows start anywhere in a line, and tiles cut at whole columns
 // wrote every 128-byte line that two of them share in parts (16,000 x 16,980 fp32: 370 us, 235 with c = 16,960, whose rows are whole
 // lines).  So a tile computes 256 columns (32 x 256 per wave) and writes, row by row, the 224 that begin with its first whole line; the
-// values go through LDS in a ring of two 32-column blocks, from which each line is taken as soon as its second block is there.
+// values go through LDS in a ring of two 32-column blocks, from which each line is taken as soon as its second block is there.  A line is 32
+// values: 128 bytes in fp32; 16-bit outputs are written in half lines, and values one by one where rows start between groups of four.
 constexpr int kWideRows = 128, kWideCols = 256, kWideStep = 224;
 
 template <int P>

@@ -15,10 +15,18 @@
 //
 // Products of fp32 tables run on the f16 matrix pipe as two planes, x 2^b = hi + lo, with a power of two per ROW that brings its
 // largest value into [2^13, 2^14): hi + lo then hold 22 bits of every value within 2^16 of the row's largest and an absolute 2^-38 of
-// it below; three products (hi hi, hi lo, lo hi) leave about 6e-8 of sum |a b|, as an fp32 sum does.  No range of values is excluded (the
-// scale stops at 2^77: a row whose largest value is below 2^-80 is held in fewer bits).  A coefficient 2^(y - M) is rounded to two planes
-// for fp32 tables and to the tables' own type for 16-bit ones; the targets', the largest terms of their sums, to two planes of either.
-// The reference exponents M are whole numbers, so every rescaling is exact.
+// it below; three products (hi hi, hi lo, lo hi; lo lo is left out) leave about 6e-8 of sum |a b|, as an fp32 sum does.  Fewer bits than fp32
+// arithmetic keeps, place by place:
+//   - rows whose largest value is below 2^-80 (the power stops at 2^77), and items whose rows are 2^100 smaller than the largest of the
+//     call (their 2^-b rides in the exponent beside the reference, and their terms below 2^-36 of the largest leave the normaliser);
+//   - where 16 rows of zeros are neighbours, rows below 2^-27 beside them (see xent_prep_kernel);
+//   - rows of more than 2^90 may overflow (a product is brought back by one side's power before the other's);
+//   - a coefficient 2^(y - M) of an fp32 table is held in two planes: 22 bits down to 2^-24 of the largest of kAside stages, an absolute 2^-34
+//     of that one below: at most 2^-22 of it in all that the 4,096 rows of those stages can lose;
+//   - a coefficient of a 16-bit table is rounded to the table's type before it meets the rows, as these are: it moves the sums by less than the
+//     rounding of the result (8,192 x 16,980 bf16: both 1.7e-3 from the definition, 2.6e-4 apart in d_rows, 9e-5 in d_table).  The targets',
+//     the largest terms of their sums, are held in two planes for every type.
+// Sums, normalisers and references are fp32.  The reference exponents M are whole numbers, so every rescaling is exact.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -174,13 +182,14 @@ __device__ __forceinline__ typename T::V read_cols(const char* lds, int plane, i
   return __builtin_bit_cast(typename T::V, c);
 }
 
-// What bounds it (measured): 4,096 x 1M x 128 fp32 takes 5.37 ms a pass, 1.17 PFLOP/s of issued products: the matrix pipe is busy in 65% of
-// its cycles, the vector ALU in 49%, at the 1.73 GHz that the card holds under them.  8,192 x 16,980 x 100 bf16: forward 81 us (pipe 46%,
-// vector ALU 50%: as many exponentials and conversions as products), backward 101 (the target branch, and its popular items' workgroups).
+// What bounds it (measured): 4,096 x 1M x 128 fp32 takes 5.45 + 5.36 ms (best of 40: 5.36 + 5.33), 1.16 PFLOP/s of issued products: the matrix
+// pipe is busy in 63% and 66% of its cycles, the vector ALU in 50%, at the 1.73 GHz that the card holds under them.  8,192 x 16,980 x 100 bf16:
+// forward 83 us (pipe 45%, vector ALU 50%: as many exponentials and conversions as products), backward 103 (pipe 37%, vector ALU 45%: the target
+// branch, and its popular items' workgroups).
 // Two workgroups of four waves on a CU, 250 registers a wave; a third does not fit.  32 x 32 x 16 products, because their accumulator
 // layout is the next product's operand layout (read_cols): the coefficients never leave the registers.  LDS reads meet no bank conflict.
 // Tried and left: results of a line of equal pieces instead of splits (5.5 -> 5.9 ms, 8,192: 135 -> 160 us), workgroups of two waves that
-// need no splits (512 x 17,000: 77 -> 95 us).
+// need no splits (512 x 17,000: 77 -> 95 us), references at the top of f16's range (kTop 13 and 15: 8,192 x 16,980 204 -> 209 and 217 us).
 //
 // The streaming kernel.  DU: the columns in use, rounded up (of rows DP wide in their image).  BWD: own rows are items.  WT: row weights of
 // either sign.  MEAN: the O sums are wanted.
@@ -234,7 +243,7 @@ __global__ void __launch_bounds__(256, 2) xent_stream_kernel(Side own, Side str,
           }
         }
       // Operands three steps (NP == 1: four or eight reads) ahead of their products: left alone, the compiler read, waited and multiplied one
-      // by one (4,096 x 1M fp32, forward: 5.55 ms; so 5.47).
+      // by one (4,096 x 1M fp32, forward: 5.55 ms; so 5.47, on one box).
       constexpr int kAhead = NP == 2 ? 6 : BWD ? 4 : 8, kReads = NP * KS * RT;
       __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
@@ -585,7 +594,7 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, 
   const bool first = (int64_t)blockIdx.x < a_blocks;
   const PrepSide s = first ? a : b;
   const int64_t row = ((int64_t)blockIdx.x - (first ? 0 : a_blocks)) * (256 / LR) + threadIdx.x / LR;
-  if (row >= s.rows_pad) return;
+  if (row >= s.rows_pad) return;      // (of whole workgroups: rows_pad is a multiple of 128)
   const int q = threadIdx.x % LR;
   bool use = row < s.rows;
   float bias = 0.f;
@@ -606,10 +615,19 @@ __global__ void __launch_bounds__(256) xent_prep_kernel(PrepSide a, PrepSide b, 
     for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
 #pragma unroll
     for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    // 2^15 2^77 and 2^23 rows stay below 2^127 in l.  A row of zeros goes as one of 2^-27: it adds nothing to O, and its coefficient should not set
-    // the reference of those that do.
-    int b = top > 0.f ? 0 : 40;
-    if (top > 0.f && top < INFINITY) b = min(77, 14 - __builtin_amdgcn_frexp_expf(top));
+    // 2^15 2^77 and 2^23 rows stay below 2^127 in l
+    const bool scaled = top > 0.f && top < INFINITY;
+    int b = scaled ? min(77, 14 - __builtin_amdgcn_frexp_expf(top)) : 0;
+    // A row of zeros adds nothing to O, and its coefficient should not set the reference of rows that do: it goes as one of the smallest row of
+    // its workgroup, or of 2^-27 among nothing but zeros.
+    __shared__ int s_b[4];
+    int most = scaled ? b : INT32_MIN;
+#pragma unroll
+    for (int o = LR; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+    if ((threadIdx.x & 63) == 0) s_b[threadIdx.x >> 6] = most;
+    __syncthreads();
+    most = max(max(s_b[0], s_b[1]), max(s_b[2], s_b[3]));
+    if (top == 0.f) b = most > INT32_MIN ? most : 40;
     inv = ldexpf(1.f, -b);
     shift = (float)b;
     f16x8 hi, lo;
@@ -1029,7 +1047,7 @@ inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // 17,000 x 100 fp32 (4 own tiles, 266 stages): 106 / 84 / 74 / 77 / 85 / 90 with 16 / 32 / 54 / 89 / 133 / 256; 1,000 x 50,021 bf16 (8, 782):
 // 141 / 113 / 109 / 120 / 145 with 16 / 32 / 64 / 89 / 256.  Backward, the same two (133, 8): 90 / 80 / 74 / 78 / 80 / 89 with 1 / 2 / 3 / 4 /
 // 6 / 8; (391, 16): 110 / 105 / 110 / 113 / 142 with 1 / 2 / 3 / 4 / 8; 2,048 x 4,000 fp32 (32, 32): 236 / 153 / 109 / 92 / 87 / 102 with 1 / 2 / 4 /
-// 8 / 16 / 32.
+// 8 / 16 / 32.  These three shapes are all it rests on.
 inline int splits_for(int64_t own_tiles, int64_t stages, bool backward) {
   int best = 1;
   int64_t least = INT64_MAX;
@@ -1087,7 +1105,7 @@ Layout layout(int64_t n, int64_t c, int d, int dtype, bool grad) {
 
 // Up to four rows take the kernels of a few rows: one row of 17,000 x 100 fp32 24 us (47 through images and the matrix pipe), four 35 (48),
 // of 1M x 128 330 and 403 (574); in 16 bits, where the table is half the bytes and the matrix pipe needs a third of the products, four
-// rows only of a smaller table: 35 (38) at 17,000, but 471 (323) at 1M.
+// rows only of a smaller table: 35 (38) at 17,000, but 471 (323) at 1M.  131,072 is a place between these two, not a measured one.
 constexpr int kFewRows = 4;
 inline bool few_rows(int64_t n, int64_t c, int32_t dtype) { return n == 1 || (n <= kFewRows && (dtype == NNCF_F32 || c < 131072)); }
 
