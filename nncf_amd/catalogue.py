@@ -73,7 +73,8 @@ def softmax_xent(rows, table, target, bias=None, weight=None, scale=1.0, reducti
 
     target (int32): a negative one takes the row out (loss 0, lse 0, gradient 0, whatever its values); one >= c makes the loss and
     the gradients NaN.  bias [c] float32: -inf leaves an item out (its row is not used); a row whose target is left out has loss
-    +inf and no gradient.  weight [n] float32: any finite value."""
+    +inf and no gradient.  weight [n] float32: any finite value (a row that is not finite reaches the table's gradient at weight 0 too).
+    fp32 magnitudes: include/nncf_hip.h."""
     _matrix(rows, "rows", _DTYPES)
     _matrix(table, "table", _DTYPES)
     n, d = rows.shape

@@ -58,7 +58,7 @@ __device__ __forceinline__ uint64_t codes8(const float* x, Coder c) {
   return r;
 }
 
-// Bound by its bytes: 1M x 128 fp32 134 us, 644 MB at 4.8 TB/s (a copy of 1 GiB: 5.2); back to fp32 121 us, 5.3 TB/s.
+// Bound by its bytes: 1M x 128 fp32 135 us, 644 MB at 4.8 TB/s (a copy of 1 GiB: 5.2); back to fp32 125 us, 5.2 TB/s.
 // One row per LR lanes, 8 columns a lane and step.  Rows of one step (LR = 8, 16) stay in registers between the two uses of a
 // value; longer ones are read twice, the second time from a cache.
 template <class E, int LR, bool ONE>
@@ -138,7 +138,7 @@ struct Scores {
 // (32 WM) x (32 WC) outputs per wave, RW x 2 waves; KB codes of every row a stage, two stages in turn, filled from global memory without a
 // register (1 KB per wave and instruction).  Chunks of 16 bytes are placed so that the 32 rows of an operand read meet every bank alike.
 // 128 codes a stage are whole lines: 2,000 x 16,384 x 4,096 took 165 us in halves of lines with tiles of 128 x 256, whether one stage lay
-// ahead or two, and takes 147 (best of 40: 129) in whole ones with 256 x 256: 1.8-2.1 POP/s, the pipe busy in 57% of its cycles (44% before).
+// ahead or two, and takes 154 (best of 40: 132) in whole ones with 256 x 256: 1.7-2.0 POP/s, the pipe busy in 57% of its cycles (44% before).
 typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 

@@ -182,10 +182,10 @@ __device__ __forceinline__ typename T::V read_cols(const char* lds, int plane, i
   return __builtin_bit_cast(typename T::V, c);
 }
 
-// What bounds it (measured): 4,096 x 1M x 128 fp32 takes 5.45 + 5.36 ms (best of 40: 5.36 + 5.33), 1.16 PFLOP/s of issued products: the matrix
-// pipe is busy in 63% and 66% of its cycles, the vector ALU in 50%, at the 1.73 GHz that the card holds under them.  8,192 x 16,980 x 100 bf16:
-// forward 83 us (pipe 45%, vector ALU 50%: as many exponentials and conversions as products), backward 103 (pipe 37%, vector ALU 45%: the target
-// branch, and its popular items' workgroups).
+// What bounds it (measured): 4,096 x 1M x 128 fp32 takes 5.63 + 5.57 ms (best of 40: 5.57 + 5.54; on another box 5.36 + 5.33), 1.12 PFLOP/s of
+// issued products: the matrix pipe is busy in 63% and 66% of its cycles, the vector ALU in 50%, at the 1.73 GHz that the card holds under them.
+// 8,192 x 16,980 x 100 bf16: forward 85 us (pipe 45%, vector ALU 50%: as many exponentials and conversions as products), backward 106 (pipe 37%,
+// vector ALU 45%: the target branch, and its popular items' workgroups).
 // Two workgroups of four waves on a CU, 250 registers a wave; a third does not fit.  32 x 32 x 16 products, because their accumulator
 // layout is the next product's operand layout (read_cols): the coefficients never leave the registers.  LDS reads meet no bank conflict.
 // Tried and left: results of a line of equal pieces instead of splits (5.5 -> 5.9 ms, 8,192: 135 -> 160 us), workgroups of two waves that
