@@ -1,6 +1,6 @@
 #!/bin/bash
 # profiles/traffic.json only (after a change of csrc/ that does not change what the kernels do -- a comment): the kernel traces and
-# FETCH / WRITE passes it is made of; on the GPU box, from the repo root.  Copy gpurun_out/traffic_*.txt to profiles/ and
+# FETCH / WRITE passes it is made of; on a machine with the GPU, from the repo root.  Copy gpurun_out/traffic_*.txt to profiles/ and
 # gpurun_out/traffic_traffic.json to profiles/traffic.json: the passes of a collection of all benchmarks (r06_*) stay as they are.
 set -u
 TAG=${1:-traffic}
